@@ -132,6 +132,10 @@ SIGNATURES = {
     "ogl_sample_blocks_small_fill": (_i, [_p, _p, _p, _i, _i, C.c_uint64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p]),
     "ogl_stage_segments": (_i, [_i, _p, _p, _p, _p, _p, _i64, _p]),
     "ogl_fuse_block_segments": (_i, [_p, _p, _i, _p, _p, _i, _p, _p]),
+    "ogl_quant_rows_workspace_bytes": (_i64, [_i64, _i64, _i]),
+    "ogl_quant_rows_write": (_i, [_p, _i64, _i, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p]),
+    "ogl_linear_i8": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p, _i, _p, _i, _p, _i64, _i, _p]),
+    "ogl_quant_rows_read": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _p, _i64, _p, _i64, _i, _p]),
 }
 
 class RecSeg(C.Structure):

@@ -3266,3 +3266,204 @@ def cross_entropy(logits, labels, reduction="mean"):
     if reduction == "sum":
         return rows.sum()
     raise ValueError("unknown reduction %r" % (reduction,))
+
+
+# --------------------------------------------------------------------------------------------
+# row operators: rows kept in 8 bits
+# --------------------------------------------------------------------------------------------
+_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_ROW_FORMATS = {"int8": (torch.int8, 0), "e4m3": (torch.float8_e4m3fn, 1)}
+
+
+def _row_device(what, *tensors):
+    """The one GPU that all of ``tensors`` (None: left out) live on; work is enqueued on THAT device's current stream."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("%s: ogl_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback" % what)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError("%s: tensors on %s and %s" % (what, dev, t.device))
+    return dev
+
+
+def _row_launch(dev, name, fn, *args, meta=None):
+    """``_launch`` on ``dev``'s current stream, whichever device is current."""
+    if dev.index == torch._C._cuda_getDevice():
+        _launch(name, fn, *args, _stream(), meta=meta)
+    else:
+        with torch.cuda.device(dev):
+            _launch(name, fn, *args, _stream(), meta=meta)
+
+
+def _row_mat(what, x):
+    """A 2-D tensor of float32 / bfloat16 / float16 rows, contiguous along the columns (copied if it is not)."""
+    if x.dim() != 2:
+        raise ValueError("%s: expected a 2-D tensor, got shape %s" % (what, tuple(x.shape)))
+    if x.dtype not in _ROW_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 rows, not %s" % (what, x.dtype))
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _row_ids(what, ids, dev):
+    if ids.dtype != torch.int64 or ids.dim() != 1 or not ids.is_contiguous():
+        raise ValueError("%s: ids must be a contiguous 1-D int64 tensor" % what)
+    return ids
+
+
+def _row_empty(rows, cols, dtype, device):
+    """[rows, cols] view of an allocation with ``padded_ld`` columns (``empty_mat`` for any row type)."""
+    return torch.empty((rows, padded_ld(cols)), dtype=dtype, device=device)[:, :cols]
+
+
+class QuantRows:
+    """Rows kept in 8 bits: ``codes`` [n, ld] (int8 or float8_e4m3fn, contiguous, 64-byte aligned, ld a multiple of 64, ZEROS behind column
+    ``width``) and float32 ``scales`` [n, ceil(width / group)], one for every ``group`` columns (a multiple of 8; None or >= width: one a row).
+    A value is ``code * scale``.  ``quant_rows`` allocates one, ``quant_rows_write`` fills rows, ``quant_rows_read`` gathers them back and
+    ``linear_int8`` multiplies them as they are kept (int8, one scale a row)."""
+
+    __slots__ = ("codes", "scales", "width", "group", "format")
+
+    def __init__(self, codes, scales, width, group=None):
+        width = int(width)
+        group = width if group is None else min(int(group), width)
+        formats = {dt: code for dt, code in _ROW_FORMATS.values()}
+        if codes.dim() != 2 or codes.dtype not in formats or not codes.is_contiguous() or codes.shape[1] % 64:
+            raise ValueError("QuantRows: codes must be contiguous int8 or float8_e4m3fn rows of a multiple of 64 bytes")
+        if not 1 <= width <= codes.shape[1]:
+            raise ValueError("QuantRows: width %d does not fit rows of %d bytes" % (width, codes.shape[1]))
+        if group < 1 or (group < width and group % 8):
+            raise ValueError("QuantRows: a group is a multiple of 8 columns or the whole row, not %d" % group)
+        if scales.dtype != torch.float32 or not scales.is_contiguous() or tuple(scales.shape) != (codes.shape[0], -(-width // group)):
+            raise ValueError("QuantRows: scales must be contiguous float32 [%d, %d]" % (codes.shape[0], -(-width // group)))
+        if codes.device != scales.device:
+            raise ValueError("QuantRows: codes on %s, scales on %s" % (codes.device, scales.device))
+        if codes.numel() and codes.data_ptr() % 64:
+            raise ValueError("QuantRows: codes must be 64-byte aligned")
+        self.codes, self.scales, self.width, self.group, self.format = codes, scales, width, group, formats[codes.dtype]
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.width)
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + 4 * self.scales.numel()
+
+
+def quant_rows(n, width, group=None, fmt="int8", device="cuda"):
+    """An empty cache of ``n`` rows of ``width`` columns in 8 bits (rows read as zeros until they are written)."""
+    if fmt not in _ROW_FORMATS:
+        raise ValueError("quant_rows: unknown format %r (int8, e4m3)" % (fmt,))
+    n, width = int(n), int(width)
+    if n < 0 or width < 1:
+        raise ValueError("quant_rows: n >= 0 rows of width >= 1, not %d x %d" % (n, width))
+    g = width if group is None else min(int(group), width)
+    if g < 1:
+        raise ValueError("quant_rows: a group has at least one column, not %d" % g)
+    codes = torch.zeros((n, (width + 63) // 64 * 64), dtype=torch.int8, device=device).view(_ROW_FORMATS[fmt][0])
+    return QuantRows(codes, torch.zeros((n, -(-width // g)), dtype=torch.float32, device=device), width, group)
+
+
+def quant_rows_write(cache, x, slots=None, start=0):
+    """Quantises the rows of ``x`` [m, width] (float32 / bfloat16 / float16) into ``cache`` at ``slots`` (int64 [m]; entries outside the cache
+    are skipped, of a repeated slot the last row stands) or at rows ``start`` ..; each group of columns with the scale max|x| / 127 (int8) or
+    / 448 (e4m3), codes rounded to nearest even from the exact quotient.  A group with an infinity or NaN reads back as NaN.  No gradient."""
+    what = "quant_rows_write"
+    x = _row_mat(what, x)
+    dev = _row_device(what, cache.codes, x, slots)
+    m, n = x.shape[0], cache.shape[0]
+    if x.shape[1] != cache.width:
+        raise ValueError("%s: rows of %d columns into a cache of %d" % (what, x.shape[1], cache.width))
+    start = int(start)
+    if slots is not None:
+        if start != 0:
+            raise ValueError("%s: slots or start, not both" % what)
+        if _row_ids(what, slots, dev).numel() != m:
+            raise ValueError("%s: %d slots for %d rows" % (what, slots.numel(), m))
+    elif start < 0 or start + m > n:
+        raise ValueError("%s: rows %d .. %d of a cache of %d" % (what, start, start + m, n))
+    if m == 0 or n == 0:
+        return cache
+    h = _lib.lib()
+    nb = h.ogl_quant_rows_workspace_bytes(m, n, slots is not None)
+    ws = torch.empty(nb // 4, dtype=torch.int32, device=dev) if nb else None
+    _row_launch(dev, "ogl_quant_rows_write", h.ogl_quant_rows_write, _ptr(x), _ld(x), _ROW_TYPES[x.dtype], m, cache.width, _ptr(slots), start,
+                _ptr(cache.codes), cache.codes.shape[1], cache.format, _ptr(cache.scales), n, cache.group, _ptr(ws), nb,
+                meta=dict(m=m, width=cache.width))
+    return cache
+
+
+def quant_rows_read(cache, rows=None, dtype=torch.float32):
+    """``code * scale`` of the cache's rows ``rows`` (int64 [m]; ids outside the cache yield zero rows; None: every row) as ``dtype``."""
+    what = "quant_rows_read"
+    if dtype not in _ROW_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 values, not %s" % (what, dtype))
+    dev = _row_device(what, cache.codes, rows)
+    m = cache.shape[0] if rows is None else _row_ids(what, rows, dev).numel()
+    out = _row_empty(m, cache.width, dtype, dev)
+    if m:
+        _row_launch(dev, "ogl_quant_rows_read", _lib.lib().ogl_quant_rows_read, _ptr(cache.codes), cache.codes.shape[1], cache.format,
+                    _ptr(cache.scales), cache.shape[0], cache.width, cache.group, _ptr(rows), m, _ptr(out), out.stride(0), _ROW_TYPES[dtype],
+                    meta=dict(m=m, width=cache.width))
+    return out
+
+
+def quantize_rows(x, group=None, fmt="int8"):
+    """``x`` [m, width] as a new ``QuantRows``."""
+    x = _row_mat("quantize_rows", x)
+    if x.shape[1] < 1:
+        raise ValueError("quantize_rows: rows without columns")
+    _row_device("quantize_rows", x)
+    return quant_rows_write(quant_rows(x.shape[0], x.shape[1], group, fmt, x.device), x)
+
+
+def _row_int8(what, q):
+    if not isinstance(q, QuantRows) or q.format != 0 or q.scales.shape[1] != 1:
+        raise ValueError("%s: int8 rows with one scale a row (quantize_rows(x)) are multiplied" % what)
+    return q
+
+
+def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
+    """``act((sx sw^T) * (x @ w^T) + bias)`` of rows kept in int8: ``x`` a ``QuantRows`` of tokens or vertices (``x_rows``: int64 ids of the rows to
+    take; ids outside it count as zero rows) or a float matrix, which is quantised row by row first; ``w`` the ``QuantRows`` of a weight
+    [out_features, in_features].  The sum is exact, the rest float32, the result ``dtype``.  Inference only: there is no gradient."""
+    what = "linear_int8"
+    _row_int8(what, w)
+    if dtype not in _ROW_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16 results, not %s" % (what, dtype))
+    if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad) or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("%s is inference only (run it under torch.no_grad())" % what)
+    if isinstance(x, torch.Tensor):
+        if x_rows is not None:
+            raise ValueError("%s: x_rows selects rows of a QuantRows" % what)
+        x = quantize_rows(x)
+    _row_int8(what, x)
+    N, K = w.shape
+    if x.width != K:
+        raise ValueError("%s: rows of %d columns, a weight of %d" % (what, x.width, K))
+    if K >= 131072:
+        raise ValueError("%s: at most 131071 columns (the sum is kept in 32 bits)" % what)
+    if bias is not None and (bias.dim() != 1 or bias.numel() != N or bias.dtype != torch.float32):
+        raise ValueError("%s: the bias must be float32 [%d]" % (what, N))
+    dev = _row_device(what, x.codes, w.codes, bias, x_rows)
+    M = x.shape[0] if x_rows is None else _row_ids(what, x_rows, dev).numel()
+    y = _row_empty(M, N, dtype, dev)
+    if M == 0 or N == 0:
+        return y
+    if x.shape[0] == 0:
+        raise ValueError("%s: rows of an empty table" % what)
+    b = bias.contiguous() if bias is not None else None
+    _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, _ptr(x.codes), x.codes.shape[1], _ptr(x.scales), _ptr(x_rows), x.shape[0], M, K,
+                _ptr(w.codes), w.codes.shape[1], _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), y.stride(0), _ROW_TYPES[dtype],
+                meta=dict(M=M, N=N, K=K))
+    return y
