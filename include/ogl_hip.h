@@ -831,6 +831,20 @@ int ogl_quant_rows_read(const void* codes, int64_t ldc, int format, const float*
 int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const int64_t* rows, int64_t nrows, int64_t M, int K, const void* w, int64_t ldw,
                   const float* sw, int N, const float* bias, int relu, void* y, int64_t ldy, int y_type, ogl_stream_t stream);
 
+/* Group norm with an activation, channels last.  x [B, L, C]: element (b, l, c) at x[b xb + l xl + c]; G groups of C / G channels.
+ *   mean, var over the L C / G values of a (sample, group);  rstd = 1 / sqrt(var + eps);  y = act((x - mean) rstd w[c] + b[c])
+ * w, b (nullable: 1 and 0) in p_type, which is OGL_F32 or x_type; y, dy, dx in x_type; mean, rstd float32 [B, G] (both or neither in the forward).
+ * The backward writes dx (nullable), dw and db (nullable, [C] in p_type); statistics and sums are float32 in a fixed order (no atomics).
+ * L <= 2^30, C <= 2^22.  An empty x (B or L of 0): the forward has nothing to do, the backward returns OGL_EINVAL (its sums are zeros). */
+enum { OGL_ACT_NONE = 0, OGL_ACT_RELU = 1, OGL_ACT_SILU = 2, OGL_ACT_GELU = 3 };
+int64_t ogl_group_norm_workspace_bytes(int64_t B, int64_t L, int C, int G, int x_type, int backward);
+int ogl_group_norm_fwd(const void* x, int64_t xb, int64_t xl, int x_type, int64_t B, int64_t L, int C, int G, const void* w, const void* b, int p_type,
+                       float eps, int act, void* y, int64_t yb, int64_t yl, float* mean, float* rstd, void* workspace, int64_t workspace_bytes,
+                       ogl_stream_t stream);
+int ogl_group_norm_bwd(const void* dy, int64_t gb, int64_t gl, const void* x, int64_t xb, int64_t xl, int x_type, int64_t B, int64_t L, int C, int G,
+                       const void* w, const void* b, int p_type, int act, const float* mean, const float* rstd, void* dx, int64_t dxb, int64_t dxl,
+                       void* dw, void* db, void* workspace, int64_t workspace_bytes, ogl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

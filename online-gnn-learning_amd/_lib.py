@@ -134,6 +134,9 @@ SIGNATURES = {
     "ogl_fuse_block_segments": (_i, [_p, _p, _i, _p, _p, _i, _p, _p]),
     "ogl_quant_rows_workspace_bytes": (_i64, [_i64, _i64, _i]),
     "ogl_quant_rows_write": (_i, [_p, _i64, _i, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p]),
+    "ogl_group_norm_workspace_bytes": (_i64, [_i64, _i64, _i, _i, _i, _i]),
+    "ogl_group_norm_fwd": (_i, [_p, _i64, _i64, _i, _i64, _i64, _i, _i, _p, _p, _i, _f, _i, _p, _i64, _i64, _p, _p, _p, _i64, _p]),
+    "ogl_group_norm_bwd": (_i, [_p, _i64, _i64, _p, _i64, _i64, _i, _i64, _i64, _i, _i, _p, _p, _i, _i, _p, _p, _p, _i64, _i64, _p, _p, _p, _i64, _p]),
     "ogl_linear_i8": (_i, [_p, _i64, _p, _p, _i64, _i64, _i, _p, _i64, _p, _i, _p, _i, _p, _i64, _i, _p]),
     "ogl_quant_rows_read": (_i, [_p, _i64, _i, _p, _i64, _i, _i, _p, _i64, _p, _i64, _i, _p]),
 }

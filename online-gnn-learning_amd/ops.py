@@ -3467,3 +3467,108 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
                 _ptr(w.codes), w.codes.shape[1], _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), y.stride(0), _ROW_TYPES[dtype],
                 meta=dict(M=M, N=N, K=K))
     return y
+
+
+# --------------------------------------------------------------------------------------------
+# row operators: group norm with an activation, channels last
+# --------------------------------------------------------------------------------------------
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _norm_view(x):
+    """``x`` [B, *spatial, C] as [B, L, C] whose channels are contiguous and whose rows do not overlap (copied if they do)."""
+    B, C = x.shape[0], x.shape[-1]
+    v = x.reshape(B, x[0, ..., 0].numel() if B else 0, C) if x.dim() > 2 else x.unsqueeze(1)
+    if (C > 1 and v.stride(2) != 1) or (v.shape[1] > 1 and v.stride(1) < C) or (B > 1 and v.stride(0) < C):
+        v = v.contiguous()
+    return v
+
+
+def _norm_empty(x):
+    """A tensor like ``x`` to write: rows of a matrix padded as the package's matrices are, otherwise contiguous."""
+    return _row_empty(x.shape[0], x.shape[1], x.dtype, x.device) if x.dim() == 2 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def group_norm_fwd(x, num_groups, weight, bias, eps, act, want_stats):
+    """(y, mean, rstd) of ``ogl_group_norm_fwd`` (statistics None unless wanted); see ``group_norm``."""
+    v = _norm_view(x)
+    (B, L, C), G = v.shape, num_groups
+    y = _norm_empty(x)
+    mean = rstd = None
+    if want_stats:
+        mean, rstd = torch.empty((2, B, G), dtype=torch.float32, device=x.device)
+    if B and L:
+        yv = _norm_view(y)
+        h, t = _lib.lib(), _ROW_TYPES[x.dtype]
+        p = weight if weight is not None else bias
+        nb = h.ogl_group_norm_workspace_bytes(B, L, C, G, t, 0)
+        ws = torch.empty(nb // 4, dtype=torch.float32, device=x.device) if nb > 0 else None
+        _row_launch(x.device, "ogl_group_norm_fwd", h.ogl_group_norm_fwd, _ptr(v), v.stride(0), v.stride(1), t, B, L, C, G, _ptr(weight), _ptr(bias),
+                    0 if p is None else _ROW_TYPES[p.dtype], eps, act, _ptr(y), yv.stride(0), yv.stride(1), _ptr(mean), _ptr(rstd), _ptr(ws), max(nb, 0),
+                    meta=dict(B=B, L=L, C=C, G=G))
+    return y, mean, rstd
+
+
+def group_norm_bwd(dy, x, num_groups, weight, bias, mean, rstd, act, want_dx=True, want_dw=True, want_db=True):
+    """(dx, dw, db) of ``ogl_group_norm_bwd``; None where not wanted."""
+    v, g = _norm_view(x), _norm_view(dy)
+    (B, L, C), G = v.shape, num_groups
+    p = weight if weight is not None else bias
+    dx = _norm_empty(x) if want_dx else None
+    dw = torch.empty(C, dtype=p.dtype, device=x.device) if want_dw else None
+    db = torch.empty(C, dtype=p.dtype, device=x.device) if want_db else None
+    if B == 0 or L == 0:
+        return dx, dw.zero_() if want_dw else None, db.zero_() if want_db else None
+    dv = _norm_view(dx) if want_dx else v
+    h, t = _lib.lib(), _ROW_TYPES[x.dtype]
+    nb = h.ogl_group_norm_workspace_bytes(B, L, C, G, t, 1)
+    ws = torch.empty(max(nb, 8) // 4, dtype=torch.float32, device=x.device)
+    _row_launch(x.device, "ogl_group_norm_bwd", h.ogl_group_norm_bwd, _ptr(g), g.stride(0), g.stride(1), _ptr(v), v.stride(0), v.stride(1), t, B, L, C, G,
+                _ptr(weight), _ptr(bias), 0 if p is None else _ROW_TYPES[p.dtype], act, _ptr(mean), _ptr(rstd), _ptr(dx), dv.stride(0), dv.stride(1),
+                _ptr(dw), _ptr(db), _ptr(ws), ws.numel() * 4, meta=dict(B=B, L=L, C=C, G=G))
+    return dx, dw, db
+
+
+class _GroupNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, eps, act):
+        y, mean, rstd = group_norm_fwd(x, num_groups, weight, bias, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.num_groups, ctx.act = num_groups, act
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        return (*group_norm_bwd(dy, x, ctx.num_groups, weight, bias, mean, rstd, ctx.act, need[0], need[1], need[2]), None, None, None)
+
+
+def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
+    """``act(group_norm(x) * weight + bias)``, channels LAST: ``x`` [B, *spatial, C] in float32 / bfloat16 / float16, statistics over the positions of
+    a sample and the C / num_groups channels of a group (a matrix [n, C]: over the channels of its row).  ``weight`` / ``bias`` [C] of the type of x
+    or float32; ``activation`` None, 'relu', 'silu' or 'gelu' (x Phi(x)).  Statistics and sums are float32, each result is rounded once.
+    Differentiable (once) w.r.t. x, weight and bias; results do not depend on the run (no atomics)."""
+    what = "group_norm"
+    if x.dim() < 2:
+        raise ValueError("%s: expected [B, *spatial, C], got shape %s" % (what, tuple(x.shape)))
+    if x.dtype not in _ROW_TYPES:
+        raise ValueError("%s: float32, bfloat16 or float16, not %s" % (what, x.dtype))
+    C, num_groups = x.shape[-1], int(num_groups)
+    if C < 1 or num_groups < 1 or C % num_groups:
+        raise ValueError("%s: %d channels in %d groups" % (what, C, num_groups))
+    if activation not in ACTIVATIONS:
+        raise ValueError("%s: unknown activation %r (None, 'relu', 'silu', 'gelu')" % (what, activation))
+    if not eps >= 0:
+        raise ValueError("%s: eps must not be negative" % what)
+    for p in (weight, bias):
+        if p is not None and (p.dim() != 1 or p.numel() != C or p.dtype not in (torch.float32, x.dtype) or not p.is_contiguous()):
+            raise ValueError("%s: weight and bias must be contiguous [%d] of float32 or %s" % (what, C, x.dtype))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("%s: weight and bias of different types" % what)
+    _row_device(what, x, weight, bias)
+    act = ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _GroupNormFn.apply(x, weight, bias, num_groups, float(eps), act)
+    return group_norm_fwd(x, num_groups, weight, bias, float(eps), act, False)[0]

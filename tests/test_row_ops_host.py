@@ -116,3 +116,45 @@ def test_linear_c_entry_checks_its_arguments():
                dict(x=p + 16), dict(w=p + 16), dict(y=p + 2), dict(y=p + 1, t=1)]:
         assert call(**kw) == -1, kw
     assert call(M=0) == 0 and call(N=0) == 0
+
+
+def test_group_norm_refuses():
+    x = torch.zeros(4, 12)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ops.group_norm(x, 3)
+    for a, kw in [((torch.zeros(12), 3), {}), ((x, 5), {}), ((x, 0), {}), ((x.double(), 3), {}), ((x, 3), dict(activation="tanh")), ((x, 3), dict(eps=-1.0)),
+                  ((x, 3, torch.ones(11)), {}), ((x, 3, torch.ones(12, dtype=torch.bfloat16)), {}), ((x, 3, torch.ones(24)[::2]), {}),
+                  ((x.half(), 3, torch.ones(12), torch.ones(12).half()), {}), ((torch.zeros(4, 0), 1), {})]:
+        with pytest.raises(ValueError):
+            ops.group_norm(*a, **kw)
+
+
+def test_group_norm_c_entries_check_their_arguments():
+    h = _lib.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    ok = dict(x=p, xb=12, xl=12, t=0, B=4, L=1, C=12, G=3, w=p, b=p, pt=0, eps=1e-5, act=1, y=p, yb=12, yl=12, mean=p, rstd=p, ws=p, nb=1 << 30, dy=p, dw=p, db=p)
+
+    def fwd(**kw):
+        a = dict(ok, **kw)
+        return h.ogl_group_norm_fwd(a["x"], a["xb"], a["xl"], a["t"], a["B"], a["L"], a["C"], a["G"], a["w"], a["b"], a["pt"], a["eps"], a["act"], a["y"],
+                                    a["yb"], a["yl"], a["mean"], a["rstd"], a["ws"], a["nb"], None)
+
+    def bwd(**kw):
+        a = dict(ok, **kw)
+        return h.ogl_group_norm_bwd(a["dy"], a["xb"], a["xl"], a["x"], a["xb"], a["xl"], a["t"], a["B"], a["L"], a["C"], a["G"], a["w"], a["b"], a["pt"],
+                                    a["act"], a["mean"], a["rstd"], a["y"], a["yb"], a["yl"], a["dw"], a["db"], a["ws"], a["nb"], None)
+
+    common = [dict(x=None), dict(t=3), dict(B=-1), dict(L=-1), dict(L=2 ** 31), dict(C=0), dict(G=0), dict(G=5), dict(pt=1), dict(act=4), dict(act=-1),
+              dict(xb=11), dict(L=2, xl=11), dict(yb=11), dict(C=2 ** 23, G=1, xb=2 ** 23, yb=2 ** 23), dict(x=p + 2), dict(w=p + 2), dict(rstd=None)]
+    for kw in common + [dict(y=None), dict(eps=-1.0), dict(eps=float("nan")), dict(mean=None)]:
+        assert fwd(**kw) == -1, kw
+    for kw in common + [dict(dy=None), dict(mean=None), dict(B=0), dict(L=0), dict(dw=p + 2)]:
+        assert bwd(**kw) == -1, kw
+    assert fwd(B=0) == 0 and fwd(L=0) == 0
+    assert bwd(y=None, dw=None, db=None) == 0                                  # nothing is wanted
+    assert bwd(ws=None) == -4 and bwd(nb=8) == -4
+    assert fwd(B=1, L=2000, ws=None) == -4 and fwd(B=1, L=2000, nb=8) == -4     # tiles of positions: partial sums
+    size = h.ogl_group_norm_workspace_bytes
+    assert size(4, 1, 12, 3, 0, 0) == 0 and size(4, 1, 12, 3, 0, 1) > 0 and size(1, 2000, 12, 3, 0, 0) > 0
+    assert size(4, 1, 12, 5, 0, 0) == -1 and size(0, 1, 12, 3, 0, 1) == 0
