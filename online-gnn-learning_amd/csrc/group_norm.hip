@@ -12,6 +12,7 @@
 // Statistics, sums and everything between load and store are float32.  Partial means and squared deviations are joined as such (count, mean, M2),
 // the squares taken around each thread's first value, so a mean far from zero costs no digits.  Sums run in an order fixed by the sizes: no atomics.
 #include <algorithm>
+#include <type_traits>
 #include "row_types.h"
 
 #pragma clang fp contract(off)   // products that have to cancel exactly (a group of one value) round where they are written; fma where it is meant
@@ -29,18 +30,54 @@ struct gn_args {
   float* sums;                   // [B, G, 2] behind it (tiled backward)
   int64_t B;
   int L, C, G, Cg, act, write_dx;
+  bool past;                     // y (dx) is stored past the caches
   float eps;
   // maps: windows of gw groups, nvec 16-byte pieces wide; rp positions side by side; tiles of tile_rows positions
   int gw, nw, nvec, rp, tiles, tile_rows, grid_b;
-  // rows: lanes of a team; the backward's tg groups x tr rows a block
-  int lanes, tg, tr, chunks;
-  ogl_div by_g;
+  // rows: lanes of a team, teams of a wave; the backward's wave has tg groups x rpw rows
+  int lanes, tw, tg, rpw, chunks;
+  ogl_div by_g, by_cg, by_lanes, by_tg, by_nvec, by_nw, by_tiles;
 };
 
+// A lane's team in the rows kernels: `lanes` neighbours (any number up to 64, so that few lanes of a wave are left over), tw of them a wave.
+struct gn_team {
+  int team, pos;
+  bool on;
+  __device__ __forceinline__ gn_team(const gn_args& A, int lane) {
+    team = (int)A.by_lanes.div((uint32_t)lane);
+    pos = lane - team * A.lanes;
+    on = team < A.tw;
+  }
+};
+// over a team, the same bits in every lane; every lane of the wave takes part
+__device__ __forceinline__ float gn_span_sum(float v, const gn_args& A, const gn_team& t) {
+  if ((A.lanes & (A.lanes - 1)) == 0) return row_team_sum(v, A.lanes);
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < A.lanes; o <<= 1) {
+    const float u = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane + o) * 4, __builtin_bit_cast(int, v)));
+    v += t.pos + o < A.lanes ? u : 0.f;
+  }
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane - t.pos) * 4, __builtin_bit_cast(int, v)));
+}
+
+// The normal distribution function at z, and e^(-z^2 / 2): Phi(-|z|) = erfc(x) / 2 at x = |z| / sqrt 2 by the polynomial of Abramowitz and Stegun
+// 7.1.26 in 1 / (1 + 0.3275911 x), off by at most 7.5e-8; the exponential is the one that the density needs too.  The library's erff takes both of
+// its branches in most waves: the gelu cases were bound by it.
+__device__ __forceinline__ float gn_phi(float z, float& e) {
+  e = __expf(-0.5f * z * z);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(z), 0.3275911f * 0.70710678f, 1.f));
+  float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+  p = __builtin_fmaf(t, p, 1.421413741f);
+  p = __builtin_fmaf(t, p, -0.284496736f);
+  p = __builtin_fmaf(t, p, 0.254829592f);
+  const float q = 0.5f * t * p * e;
+  return z < 0.f ? q : 1.f - q;
+}
 __device__ __forceinline__ float gn_act(float z, int act) {
+  float e;
   if (act == OGL_ACT_RELU) return z < 0.f ? 0.f : z;
   if (act == OGL_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (act == OGL_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+  if (act == OGL_ACT_GELU) return z * gn_phi(z, e);
   return z;
 }
 __device__ __forceinline__ float gn_slope(float z, int act) {
@@ -49,50 +86,44 @@ __device__ __forceinline__ float gn_slope(float z, int act) {
     const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     return s * __builtin_fmaf(z, 1.f - s, 1.f);
   }
-  if (act == OGL_ACT_GELU) return __builtin_fmaf(z * 0.39894228040143268f, __expf(-0.5f * z * z), 0.5f * (1.f + erff(z * 0.70710678118654752f)));
+  if (act == OGL_ACT_GELU) {
+    float e;
+    const float phi = gn_phi(z, e);
+    return __builtin_fmaf(z * 0.39894228040143268f, e, phi);
+  }
   return 1.f;
 }
 
-// n of V elements from p (the others 0) / to p
+// channel parameters c .. of a piece (`none` where there are none)
 template <typename T, int V>
-__device__ __forceinline__ void gn_load(const T* __restrict__ p, int n, float (&v)[V]) {
-  if (n >= V) {
-    row_load<T, V>(p, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = e < n ? (float)p[e] : 0.f;
-  }
-}
-template <typename T, int V>
-__device__ __forceinline__ void gn_store(T* __restrict__ p, int n, const float (&v)[V]) {
-  if (n >= V) {
-    row_store<T, V>(p, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (e < n) p[e] = (T)v[e];
-  }
-}
-// channel parameters c .. c + n - 1 (`none` where there are none)
-template <typename T, int V>
-__device__ __forceinline__ void gn_param(const void* p, int p_type, int c, int n, float none, float (&v)[V]) {
+__device__ __forceinline__ void gn_param(const void* p, int p_type, int c, const row_piece<T, V>& P, float none, float (&v)[V]) {
   if (!p) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = none;
   } else if (p_type == OGL_F32) {
-    gn_load<float, V>((const float*)p + c, n, v);
+    if constexpr (V == 4) {
+      row_piece<float, 4>(P.n, P.tiny).load((const float*)p + c, v);
+    } else {                                                            // eight channels of 32 bits: two pieces
+      const row_piece<float, 4> lo(P.n, P.tiny || P.n < 4), hi(P.n - 4, P.tiny);
+      float a[4], b[4];
+      lo.load((const float*)p + c, a);
+      hi.load((const float*)p + c + 4, b);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = a[e];
+        v[4 + e] = b[e];
+      }
+    }
   } else {
-    gn_load<T, V>((const T*)p + c, n, v);
+    P.load((const T*)p + c, v);
   }
 }
 
-__device__ __forceinline__ float gn_team_sum(float v, int lanes) {
-  for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o);
-  return v;
-}
+// a squared deviation that rounding took below zero; a NaN stays one
+__device__ __forceinline__ float gn_not_negative(float v) { return v < 0.f ? 0.f : v; }
 // over the whole block, the same order for every thread
 __device__ __forceinline__ float gn_block_sum(float v, float* lds) {
-  v = gn_team_sum(v, 64);
+  v = row_team_sum(v, 64);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -100,128 +131,184 @@ __device__ __forceinline__ float gn_block_sum(float v, float* lds) {
 }
 
 // ================================================================ rows ========================================================================
-// One team per (row, group); BLOCK: the team is the block.  NV pieces of V channels a lane.
-template <typename T, int V, int NV, bool BLOCK>
+// One team per group and R rows one below the other; BLOCK: the team is the block.  NV pieces of V channels a lane and row.  R: a team's loads are
+// issued together; one piece a lane in flight leaves the memory waiting.
+template <typename T, int V, int NV, int R, bool BLOCK>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
   __shared__ float lds[4];
-  const int lanes = BLOCK ? GN_THREADS : A.lanes;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int teams = GN_THREADS / lanes;
-  const int64_t first = (int64_t)blockIdx.x * teams;                 // the block's first team, then 32-bit steps from there
+  const gn_team t(A, threadIdx.x & 63);
+  const int lanes = BLOCK ? GN_THREADS : A.lanes, lane = BLOCK ? (int)threadIdx.x : t.pos;
+  const int64_t first = (int64_t)blockIdx.x * (BLOCK ? 1 : 4 * A.tw);  // the block's first team, then 32-bit steps from there
   const int64_t b0 = first / A.G;
-  const uint32_t k = (uint32_t)(first - b0 * A.G) + threadIdx.x / lanes;
+  const uint32_t k = (uint32_t)(first - b0 * A.G) + (BLOCK ? 0u : (threadIdx.x >> 6) * A.tw + t.team);
   const uint32_t up = A.by_g.div(k);
-  const int64_t b = b0 + up;
+  const int64_t b = (b0 + up) * R;
   const int g = (int)(k - up * A.G);
-  const bool live = b < A.B;                                          // (every lane stays for the shuffles)
+  const int rows = BLOCK || t.on ? (int)min((int64_t)R, max((int64_t)0, A.B - b)) : 0;   // (every lane stays for the shuffles)
   const int c0 = g * A.Cg;
-  const T* xp = (const T*)A.x + (live ? b : 0) * A.xb + c0;
-  float v[NV][V], s = 0.f;
+  const T* xp = (const T*)A.x + (rows ? b : 0) * A.xb + c0;
+  const bool tiny = A.Cg < V;
+  typename row_piece<T, V>::raw raw[R][NV];
+  float v[R][NV][V], mean[R], rstd[R];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int e0 = (j * lanes + lane) * V;
-    gn_load<T, V>(xp + e0, live ? A.Cg - e0 : 0, v[j]);
+  for (int q = 0; q < R; ++q)
 #pragma unroll
-    for (int e = 0; e < V; ++e) s += v[j][e];
-  }
-  const float inv = 1.f / (float)A.Cg;
-  const float mean = (BLOCK ? gn_block_sum(s, lds) : gn_team_sum(s, lanes)) * inv;
-  float q = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int n = A.Cg - (j * lanes + lane) * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      v[j][e] -= mean;
-      q = e < n ? __builtin_fmaf(v[j][e], v[j][e], q) : q;
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = (j * lanes + lane) * V;
+      raw[q][j] = row_piece<T, V>(q < rows ? A.Cg - e0 : 0, tiny).fetch(xp + q * A.xb + e0);
     }
+#pragma unroll
+  for (int q = 0; q < R; ++q)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) row_piece<T, V>(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny).expand(raw[q][j], v[q][j]);
+  const float inv = 1.f / (float)A.Cg;
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += v[q][j][e];
+    mean[q] = (BLOCK ? gn_block_sum(s, lds) : gn_span_sum(s, A, t)) * inv;
   }
-  const float var = (BLOCK ? gn_block_sum(q, lds) : gn_team_sum(q, lanes)) * inv;
-  const float rstd = 1.f / sqrtf(var + A.eps);
-  if (!live) return;
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    float d = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int n = A.Cg - (j * lanes + lane) * V;
+      if (n >= V) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[q][j][e] -= mean[q];
+          d = __builtin_fmaf(v[q][j][e], v[q][j][e], d);
+        }
+      } else if (n > 0) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[q][j][e] -= mean[q];
+          d = e < n ? __builtin_fmaf(v[q][j][e], v[q][j][e], d) : d;
+        }
+      }
+    }
+    rstd[q] = 1.f / sqrtf((BLOCK ? gn_block_sum(d, lds) : gn_span_sum(d, A, t)) * inv + A.eps);
+  }
   if (lane == 0 && A.mean) {
-    A.mean[b * A.G + g] = mean;
-    A.rstd[b * A.G + g] = rstd;
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+      if (q < rows) {
+        A.mean[(b + q) * A.G + g] = mean[q];
+        A.rstd[(b + q) * A.G + g] = rstd[q];
+      }
   }
   T* yp = (T*)A.y + b * A.yb + c0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e0 = (j * lanes + lane) * V, n = A.Cg - e0;
-    if (n <= 0) continue;
+    const int e0 = (j * lanes + lane) * V;
+    const row_piece<T, V> P(rows ? A.Cg - e0 : 0, tiny);
+    if (P.n <= 0) continue;
     float w[V], bb[V];
-    gn_param<T, V>(A.w, A.p_type, c0 + e0, n, 1.f, w);
-    gn_param<T, V>(A.b, A.p_type, c0 + e0, n, 0.f, bb);
+    gn_param<T, V>(A.w, A.p_type, c0 + e0, P, 1.f, w);
+    gn_param<T, V>(A.b, A.p_type, c0 + e0, P, 0.f, bb);
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[j][e] = gn_act(__builtin_fmaf(v[j][e] * rstd, w[e], bb[e]), A.act);
-    gn_store<T, V>(yp + e0, n, v[j]);
+    for (int q = 0; q < R; ++q) {
+      if (q >= rows) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[q][j][e] = gn_act(__builtin_fmaf(v[q][j][e] * rstd[q], w[e], bb[e]), A.act);
+      P.store(yp + q * A.yb + e0, v[q][j], A.past);
+    }
   }
 }
 
-// tg groups side by side x tr rows a block; block x of `chunks` takes every chunks-th set of rows, block y the next groups.  The sums over its rows
-// go to part[x][0: dz, 1: dz h][C].
-template <typename T, int V, int NV, bool BLOCK>
+// A wave has tg groups side by side and rpw rows, a block its four waves' rows; block x of `chunks` takes every chunks-th set of rows, block y the next
+// groups.  The sums over its rows go to part[x][0: dz, 1: dz h][C].
+template <typename T, int V, int NV, int R, bool BLOCK>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
   __shared__ float lds[2 * GN_THREADS];
-  const int lanes = BLOCK ? GN_THREADS : A.lanes;
-  const int lane = threadIdx.x & (lanes - 1), team = threadIdx.x / lanes;
-  const int gi = team % A.tg, ri = team / A.tg;
+  const gn_team t(A, threadIdx.x & 63);
+  const int lanes = BLOCK ? GN_THREADS : A.lanes, lane = BLOCK ? (int)threadIdx.x : t.pos;
+  const int rw = BLOCK ? 0 : (int)A.by_tg.div((uint32_t)t.team), gi = BLOCK ? 0 : t.team - rw * A.tg;
+  const int ri = BLOCK ? 0 : (int)(threadIdx.x >> 6) * A.rpw + rw, block_rows = BLOCK ? 1 : 4 * A.rpw;
   const int g = blockIdx.y * A.tg + gi;
-  const bool mine = g < A.G;
+  const bool mine = g < A.G && (BLOCK || (t.on && rw < A.rpw));
   const int c0 = (mine ? g : 0) * A.Cg;
   const float inv = 1.f / (float)A.Cg;
+  const bool tiny = A.Cg < V;
   float w[NV][V], bb[NV][V], sz[NV][V], sh[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e0 = (j * lanes + lane) * V, n = mine ? A.Cg - e0 : 0;
-    gn_param<T, V>(A.w, A.p_type, c0 + e0, n, 1.f, w[j]);
-    gn_param<T, V>(A.b, A.p_type, c0 + e0, n, 0.f, bb[j]);
+    const int e0 = (j * lanes + lane) * V;
+    const row_piece<T, V> P(mine ? A.Cg - e0 : 0, tiny);
+    gn_param<T, V>(A.w, A.p_type, c0 + e0, P, 1.f, w[j]);
+    gn_param<T, V>(A.b, A.p_type, c0 + e0, P, 0.f, bb[j]);
 #pragma unroll
     for (int e = 0; e < V; ++e) sz[j][e] = sh[j][e] = 0.f;
   }
   // every team runs the same number of rounds: the shuffles (and the block's barriers) see all of it
-  const int64_t step = (int64_t)A.chunks * A.tr;
-  for (int64_t r0 = (int64_t)blockIdx.x * A.tr; r0 < A.B; r0 += step) {
-    const int64_t b = r0 + ri;
-    const bool live = mine && b < A.B;
-    const int64_t at = live ? b : 0;
+  const int64_t step = (int64_t)A.chunks * block_rows * R;
+  for (int64_t r0 = (int64_t)blockIdx.x * block_rows * R; r0 < A.B; r0 += step) {
+    const int64_t b = r0 + ri * R;
+    const int rows = mine ? (int)min((int64_t)R, max((int64_t)0, A.B - b)) : 0;
+    const int64_t at = rows ? b : 0;
     const T* xp = (const T*)A.x + at * A.xb + c0;
     const T* gp = (const T*)A.dy + at * A.gb + c0;
-    const float mean = live ? A.mean[at * A.G + g] : 0.f, rstd = live ? A.rstd[at * A.G + g] : 0.f;
-    float h[NV][V], dz[NV][V], s1 = 0.f, s2 = 0.f;
+    typename row_piece<T, V>::raw rx[R][NV], rg[R][NV];
+    float h[R][NV][V], dz[R][NV][V], mean[R], rstd[R], s1[R], s2[R];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e0 = (j * lanes + lane) * V, n = live ? A.Cg - e0 : 0;
-      gn_load<T, V>(xp + e0, n, h[j]);
-      gn_load<T, V>(gp + e0, n, dz[j]);
-    }
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int n = live ? A.Cg - (j * lanes + lane) * V : 0;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (e < n) {
-          h[j][e] = (h[j][e] - mean) * rstd;
-          dz[j][e] *= gn_slope(__builtin_fmaf(h[j][e], w[j][e], bb[j][e]), A.act);
-          sz[j][e] += dz[j][e];
-          sh[j][e] = __builtin_fmaf(dz[j][e], h[j][e], sh[j][e]);
-          dz[j][e] *= w[j][e];
-          s1 += dz[j][e];
-          s2 = __builtin_fmaf(dz[j][e], h[j][e], s2);
-        }
-      }
-    }
-    if (A.write_dx) {
-      s1 = (BLOCK ? gn_block_sum(s1, lds) : gn_team_sum(s1, lanes)) * inv;
-      s2 = (BLOCK ? gn_block_sum(s2, lds) : gn_team_sum(s2, lanes)) * inv;
-      T* dp = (T*)A.y + at * A.yb + c0;
+    for (int q = 0; q < R; ++q) {
+      mean[q] = q < rows ? A.mean[(at + q) * A.G + g] : 0.f;
+      rstd[q] = q < rows ? A.rstd[(at + q) * A.G + g] : 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int e0 = (j * lanes + lane) * V, n = live ? A.Cg - e0 : 0;
-        if (n <= 0) continue;
-#pragma unroll
-        for (int e = 0; e < V; ++e) dz[j][e] = rstd * (dz[j][e] - __builtin_fmaf(h[j][e], s2, s1));
-        gn_store<T, V>(dp + e0, n, dz[j]);
+        const int e0 = (j * lanes + lane) * V;
+        const row_piece<T, V> P(q < rows ? A.Cg - e0 : 0, tiny);
+        rx[q][j] = P.fetch(xp + q * A.xb + e0);
+        rg[q][j] = P.fetch(gp + q * A.gb + e0);
       }
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const row_piece<T, V> P(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny);
+        P.expand(rx[q][j], h[q][j]);
+        P.expand(rg[q][j], dz[q][j]);
+      }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      s1[q] = s2[q] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)                                    // (behind a run's end dy is 0, and so is every term)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          h[q][j][e] = (h[q][j][e] - mean[q]) * rstd[q];
+          dz[q][j][e] *= gn_slope(__builtin_fmaf(h[q][j][e], w[j][e], bb[j][e]), A.act);
+          sz[j][e] += dz[q][j][e];
+          sh[j][e] = __builtin_fmaf(dz[q][j][e], h[q][j][e], sh[j][e]);
+          dz[q][j][e] *= w[j][e];
+          s1[q] += dz[q][j][e];
+          s2[q] = __builtin_fmaf(dz[q][j][e], h[q][j][e], s2[q]);
+        }
+    }
+    if (A.write_dx) {
+#pragma unroll
+      for (int q = 0; q < R; ++q) {
+        if (A.Cg == 1) rstd[q] = 0.f;                                   // a group of one value: dx is 0, not the rounding of what cancels
+        s1[q] = -(BLOCK ? gn_block_sum(s1[q], lds) : gn_span_sum(s1[q], A, t)) * inv * rstd[q];
+        s2[q] = -(BLOCK ? gn_block_sum(s2[q], lds) : gn_span_sum(s2[q], A, t)) * inv * rstd[q];
+      }
+      T* dp = (T*)A.y + at * A.yb + c0;
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int e0 = (j * lanes + lane) * V;
+          const row_piece<T, V> P(q < rows ? A.Cg - e0 : 0, tiny);
+          if (P.n <= 0) continue;
+#pragma unroll
+          for (int e = 0; e < V; ++e) dz[q][j][e] = __builtin_fmaf(dz[q][j][e], rstd[q], __builtin_fmaf(h[q][j][e], s2[q], s1[q]));
+          P.store(dp + q * A.yb + e0, dz[q][j], A.past);
+        }
     }
   }
   if (!A.part) return;
@@ -232,17 +319,19 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       float a = sz[j][e], c = sh[j][e];
-      if (A.tr > 1) {                                                  // the rows of the block, in order
+      if (!BLOCK) {                                                    // the rows of the block, in order
         __syncthreads();
         lds[threadIdx.x] = a;
         lds[GN_THREADS + threadIdx.x] = c;
         __syncthreads();
         a = c = 0.f;
-        if (ri == 0)
-          for (int q = 0; q < A.tr; ++q) {
-            a += lds[q * A.tg * lanes + threadIdx.x];
-            c += lds[GN_THREADS + q * A.tg * lanes + threadIdx.x];
-          }
+        if (ri == 0 && mine)
+          for (int wave = 0; wave < 4; ++wave)
+            for (int q = 0; q < A.rpw; ++q) {
+              const int at = wave * 64 + q * A.tg * lanes + threadIdx.x;
+              a += lds[at];
+              c += lds[GN_THREADS + at];
+            }
       }
       if (ri == 0 && mine && e0 + e < A.Cg) {
         out[e0 + e] = a;
@@ -269,16 +358,21 @@ __device__ __forceinline__ gn_place gn_where(const gn_args& A, int64_t b, int wi
   P.groups = min(A.gw, A.G - P.g0);
   P.c0 = P.g0 * A.Cg;
   P.W = P.groups * A.Cg;
-  P.j = threadIdx.x % A.nvec;
-  P.ri = threadIdx.x / A.nvec;
+  P.ri = (int)A.by_nvec.div(threadIdx.x);
+  P.j = threadIdx.x - P.ri * A.nvec;
   P.on = P.ri < A.rp;
   return P;
 }
 
-struct gn_stats_lds {
-  float mean[GN_THREADS * 8], m2[GN_THREADS * 8];                      // [rp][W]; WIDE: of a thread's values
-  int count[GN_THREADS];                                               // rows of ri; WIDE: values of the thread
+struct __align__(16) gn_stats_lds {
+  float a[GN_THREADS * 8], q[GN_THREADS * 8];                          // [rp][nvec V] sums around a pivot, then (mean, M2) of a channel; WIDE: of a thread
+  int count[GN_THREADS];                                               // WIDE: values of the thread
 };
+template <int V>
+__device__ __forceinline__ void gn_lds_put(float* p, const float (&v)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; e += 4) *(float4*)(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+}
 
 // lanes of a wave that work on one of `groups` groups together
 __device__ __forceinline__ int gn_group_lanes(int groups) {
@@ -287,50 +381,66 @@ __device__ __forceinline__ int gn_group_lanes(int groups) {
   return t;
 }
 
-// (mean, M2) of each of the block's groups over positions r0 .. r1, handed to `done(group of the window, mean, M2)` by one lane a group
+// (mean, M2) of each of the block's groups over positions r0 .. r1, handed to `done(group of the window, mean, M2)` by one lane a group.
+// NARROW: sums and squares around the channel's value at r0 (the same pivot for every thread of a channel, so they add up), a channel's mean and M2
+// from them, and the channels of a group joined around the first one's mean.
 template <typename T, int V, bool WIDE, typename F>
 __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place& P, int r0, int r1, gn_stats_lds& S, F done) {
-  const T* xp = (const T*)A.x + P.b * A.xb + P.c0;
+  const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + (int64_t)r0 * A.xl;
+  const int rows = r1 - r0;
+  const float in = 1.f / (float)rows;
   if constexpr (!WIDE) {
-    float k[V], s[V], q[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) k[e] = s[e] = q[e] = 0.f;
-    int n = 0;
     const int have = P.on ? P.W - P.j * V : 0;
     if (have > 0) {
-      for (int r = r0 + P.ri; r < r1; r += A.rp) {
-        float v[V];
-        gn_load<T, V>(xp + (int64_t)r * A.xl + P.j * V, have, v);
-        if (n == 0) {
+      float k[V], s[V], q[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) k[e] = v[e];
-        }
+      for (int e = 0; e < V; ++e) s[e] = q[e] = 0.f;
+      const row_piece<T, V> C(have, P.W < V);
+      const T* p = xp + P.j * V;
+      const typename row_piece<T, V>::raw pivot = C.fetch(p);
+      const int64_t step = (int64_t)A.rp * A.xl;
+      p += P.ri * A.xl;
+      for (int r = P.ri; r < rows; r += 8 * A.rp, p += 8 * step) {     // eight loads in flight
+        typename row_piece<T, V>::raw raw[8];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float d = v[e] - k[e];
-          s[e] += d;
-          q[e] = __builtin_fmaf(d, d, q[e]);
+        for (int u = 0; u < 8; ++u)
+          if (r + u * A.rp < rows) raw[u] = C.fetch(p + u * step);
+        if (r == P.ri) C.expand(pivot, k);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (r + u * A.rp >= rows) break;
+          float v[V];
+          C.expand(raw[u], v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float d = v[e] - k[e];
+            s[e] += d;
+            q[e] = __builtin_fmaf(d, d, q[e]);
+          }
         }
-        ++n;
       }
-      const float in = n ? 1.f / (float)n : 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (e < have) {
-          const float d = s[e] * in;
-          S.mean[P.ri * P.W + P.j * V + e] = k[e] + d;
-          S.m2[P.ri * P.W + P.j * V + e] = fmaxf(__builtin_fmaf(-d, s[e], q[e]), 0.f);
-        }
+      gn_lds_put<V>(S.a + (P.ri * A.nvec + P.j) * V, s);
+      gn_lds_put<V>(S.q + (P.ri * A.nvec + P.j) * V, q);
     }
-    if (P.on && P.j == 0) S.count[P.ri] = n;
+    __syncthreads();
+    for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {               // (entry c of position 0 is this thread's from here on)
+      float s = 0.f, q = 0.f;
+      for (int ri = 0; ri < A.rp; ++ri) {
+        s += S.a[ri * A.nvec * V + c];
+        q += S.q[ri * A.nvec * V + c];
+      }
+      const float d = s * in;
+      S.a[c] = (float)xp[c] + d;
+      S.q[c] = gn_not_negative(__builtin_fmaf(-d, s, q));
+    }
   } else {
     float k = 0.f, s = 0.f, q = 0.f;
     int n = 0;
     for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
       const int have = P.W - j * V;
-      for (int r = r0; r < r1; ++r) {
+      for (int r = 0; r < rows; ++r) {
         float v[V];
-        gn_load<T, V>(xp + (int64_t)r * A.xl + j * V, have, v);
+        row_piece<T, V>(have, false).load(xp + (int64_t)r * A.xl + j * V, v);
         if (n == 0) k = v[0];
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -343,8 +453,8 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
       }
     }
     const float d = n ? s / (float)n : 0.f;
-    S.mean[threadIdx.x] = k + d;
-    S.m2[threadIdx.x] = fmaxf(__builtin_fmaf(-d, s, q), 0.f);
+    S.a[threadIdx.x] = k + d;
+    S.q[threadIdx.x] = gn_not_negative(__builtin_fmaf(-d, s, q));
     S.count[threadIdx.x] = n;
   }
   __syncthreads();
@@ -353,52 +463,73 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
   for (int q0 = 0; q0 < P.groups; q0 += per) {
     const int g = q0 + threadIdx.x / lanes;
     const bool live = g < P.groups;
-    const int entries = live ? (WIDE ? GN_THREADS : A.rp * A.Cg) : 0;
-    const float total = (float)A.Cg * (float)(r1 - r0);
-    float mean = 0.f, m2 = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {
-      float a = 0.f;
-      for (int t = lane; t < entries; t += lanes) {
-        const int ri = WIDE ? t : t / A.Cg, at = WIDE ? t : ri * P.W + g * A.Cg + (t - ri * A.Cg);
-        const int n = S.count[ri];
-        if (n) {
-          const float d = S.mean[at] - mean;
-          a += pass == 0 ? (float)n * d : __builtin_fmaf((float)n * d, d, S.m2[at]);
+    const int at = WIDE ? 0 : g * A.Cg;
+    const float total = (float)A.Cg * (float)rows, first = live ? S.a[at] : 0.f;
+    float a = 0.f, m2 = 0.f;
+    if (live)
+      for (int c = lane; c < (WIDE ? GN_THREADS : A.Cg); c += lanes) {
+        const float n = WIDE ? (float)S.count[c] : (float)rows, d = S.a[at + c] - first;
+        if (n > 0.f) {
+          a = __builtin_fmaf(n, d, a);
+          m2 += __builtin_fmaf(n * d, d, S.q[at + c]);
         }
       }
-      a = gn_team_sum(a, lanes);
-      if (pass == 0) mean = a / total;
-      else m2 = a;
-    }
+    a = row_team_sum(a, lanes);
+    m2 = row_team_sum(m2, lanes);
+    const float mean = first + a / total;
+    m2 = gn_not_negative(__builtin_fmaf(-a / total, a, m2));
     if (live && lane == 0) done(g, mean, m2);
   }
   __syncthreads();
 }
 
-// y of positions r0 .. r1 from the window's statistics in LDS
-template <typename T, int V, bool WIDE>
-__device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& P, int r0, int r1, const float* mean, const float* rstd) {
-  const T* xp = (const T*)A.x + P.b * A.xb + P.c0;
-  T* yp = (T*)A.y + P.b * A.yb + P.c0;
+// y of positions r0 .. r1 from the window's statistics, which `stats` (called once by every thread) puts into LDS while the first loads are on their way
+template <typename T, int V, bool WIDE, typename F>
+__device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& P, int r0, int r1, const float* mean, const float* rstd, F stats) {
+  constexpr int U = 2;
+  typedef typename row_piece<T, V>::raw raw_t;
+  const int step = WIDE ? 1 : A.rp, first = r0 + (WIDE ? 0 : P.ri);
+  raw_t ahead[U];
+  if constexpr (!WIDE) {
+    const int have = P.on ? P.W - P.j * V : 0;
+    const row_piece<T, V> C(have, P.W < V);
+    const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + P.j * V;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (have > 0 && first + u * step < r1) ahead[u] = C.fetch(xp + (int64_t)(first + u * step) * A.xl);
+  }
+  stats();
   for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
+    const row_piece<T, V> C(have, P.W < V);
+    const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + j * V;
+    T* yp = (T*)A.y + P.b * A.yb + P.c0 + j * V;
     float mu[V], a[V], bb[V];
-    gn_param<T, V>(A.w, A.p_type, P.c0 + j * V, have, 1.f, a);
-    gn_param<T, V>(A.b, A.p_type, P.c0 + j * V, have, 0.f, bb);
+    gn_param<T, V>(A.w, A.p_type, P.c0 + j * V, C, 1.f, a);
+    gn_param<T, V>(A.b, A.p_type, P.c0 + j * V, C, 0.f, bb);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const int g = WIDE ? 0 : min(j * V + e, P.W - 1) / A.Cg;
+      const int g = WIDE ? 0 : (int)A.by_cg.div(min(j * V + e, P.W - 1));
       mu[e] = mean[g];
       a[e] *= rstd[g];
     }
-#pragma unroll 4
-    for (int r = r0 + (WIDE ? 0 : P.ri); r < r1; r += WIDE ? 1 : A.rp) {
-      float v[V];
-      gn_load<T, V>(xp + (int64_t)r * A.xl + j * V, have, v);
+    for (int r = first; r < r1; r += U * step) {
+      raw_t raw[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = gn_act(__builtin_fmaf(v[e] - mu[e], a[e], bb[e]), A.act);
-      gn_store<T, V>(yp + (int64_t)r * A.yl + j * V, have, v);
+      for (int u = 0; u < U; ++u) {
+        if (!WIDE && r == first) raw[u] = ahead[u];
+        else if (r + u * step < r1) raw[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (r + u * step >= r1) break;
+        float v[V];
+        C.expand(raw[u], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = gn_act(__builtin_fmaf(v[e] - mu[e], a[e], bb[e]), A.act);
+        C.store(yp + (int64_t)(r + u * step) * A.yl, v, A.past);
+      }
     }
   }
 }
@@ -408,29 +539,30 @@ template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
   __shared__ gn_stats_lds S;
   __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
-  const int64_t b = blockIdx.x / A.nw;
-  const gn_place P = gn_where(A, b, (int)(blockIdx.x - b * A.nw), 0);
+  const int64_t b = A.by_nw.div(blockIdx.x);
+  const gn_place P = gn_where(A, b, (int)(blockIdx.x - (uint32_t)b * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
-  gn_block_stats<T, V, WIDE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
-    const float r = 1.f / sqrtf(m2 * inv + A.eps);
-    mean[g] = mu;
-    rstd[g] = r;
-    if (A.mean) {
-      A.mean[b * A.G + P.g0 + g] = mu;
-      A.rstd[b * A.G + P.g0 + g] = r;
-    }
+  gn_apply_rows<T, V, WIDE>(A, P, 0, A.L, mean, rstd, [&]() {
+    gn_block_stats<T, V, WIDE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
+      const float r = 1.f / sqrtf(m2 * inv + A.eps);
+      mean[g] = mu;
+      rstd[g] = r;
+      if (A.mean) {
+        A.mean[b * A.G + P.g0 + g] = mu;
+        A.rstd[b * A.G + P.g0 + g] = r;
+      }
+    });
   });
-  gn_apply_rows<T, V, WIDE>(A, P, 0, A.L, mean, rstd);
 }
 
 // tiles of positions: part[(b, group), tile] = (mean, M2)
 template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_stats(gn_args A) {
   __shared__ gn_stats_lds S;
-  const int64_t u = blockIdx.x / A.tiles;
+  const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
-  const int64_t b = u / A.nw;
-  const gn_place P = gn_where(A, b, (int)(u - b * A.nw), tile);
+  const int64_t b = A.by_nw.div(u);
+  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
   gn_block_stats<T, V, WIDE>(A, P, r0, r1, S, [&](int g, float mu, float m2) {
     float2* o = (float2*)A.part + (b * A.G + P.g0 + g) * A.tiles + tile;
@@ -440,106 +572,143 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_stats(gn_args A) {
 template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_apply(gn_args A) {
   __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
-  const int64_t u = blockIdx.x / A.tiles;
+  const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
-  const int64_t b = u / A.nw;
-  const gn_place P = gn_where(A, b, (int)(u - b * A.nw), tile);
-  const int lanes = gn_group_lanes(P.groups);
-  const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
-  const float total = (float)A.Cg * (float)A.L;
-  for (int q0 = 0; q0 < P.groups; q0 += per) {
-    const int g = q0 + threadIdx.x / lanes;
-    const bool live = g < P.groups;
-    const float2* o = (const float2*)A.part + (b * A.G + P.g0 + (live ? g : 0)) * A.tiles;
-    float mu = 0.f, m2 = 0.f;
-    for (int pass = 0; pass < 2; ++pass) {
-      float a = 0.f;
+  const int64_t b = A.by_nw.div(u);
+  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
+  const int r0 = tile * A.tile_rows;
+  gn_apply_rows<T, V, WIDE>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd, [&]() {
+    const int lanes = gn_group_lanes(P.groups);
+    const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
+    const float total = (float)A.Cg * (float)A.L;
+    for (int q0 = 0; q0 < P.groups; q0 += per) {
+      const int g = q0 + threadIdx.x / lanes;
+      const bool live = g < P.groups;
+      const float2* o = (const float2*)A.part + (b * A.G + P.g0 + (live ? g : 0)) * A.tiles;
+      const float first = o[0].x;                                        // (the tiles' means lie near each other: sums around the first one's)
+      float a = 0.f, m2 = 0.f;
+#pragma unroll 4
       for (int t = lane; t < A.tiles; t += lanes) {
         const float2 v = o[t];
-        const float n = (float)A.Cg * (float)min(A.tile_rows, A.L - t * A.tile_rows), d = v.x - mu;
-        a += pass == 0 ? n * d : __builtin_fmaf(n * d, d, v.y);
+        const float n = (float)A.Cg * (float)min(A.tile_rows, A.L - t * A.tile_rows), d = v.x - first;
+        a = __builtin_fmaf(n, d, a);
+        m2 += __builtin_fmaf(n * d, d, v.y);
       }
-      a = gn_team_sum(a, lanes);
-      if (pass == 0) mu = a / total;
-      else m2 = a;
-    }
-    if (live && lane == 0) {
-      const float r = 1.f / sqrtf(m2 / total + A.eps);
-      mean[g] = mu;
-      rstd[g] = r;
-      if (A.mean && tile == 0) {
-        A.mean[b * A.G + P.g0 + g] = mu;
-        A.rstd[b * A.G + P.g0 + g] = r;
+      a = row_team_sum(a, lanes);
+      m2 = row_team_sum(m2, lanes);
+      const float mu = first + a / total;
+      m2 = gn_not_negative(__builtin_fmaf(-a / total, a, m2));
+      if (live && lane == 0) {
+        const float r = 1.f / sqrtf(m2 / total + A.eps);
+        mean[g] = mu;
+        rstd[g] = r;
+        if (A.mean && tile == 0) {
+          A.mean[b * A.G + P.g0 + g] = mu;
+          A.rstd[b * A.G + P.g0 + g] = r;
+        }
       }
     }
-  }
-  __syncthreads();
-  const int r0 = tile * A.tile_rows;
-  gn_apply_rows<T, V, WIDE>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd);
+    __syncthreads();
+  });
 }
 
 // what the backward keeps of a thread's channels
 template <int V>
 struct gn_cols {
-  float mu[V], rs[V], w[V], b[V];
+  float mu[V], rs[V], w[V], a[V], b[V];                                // a = rs w: z = (x - mu) a + b
 };
 template <typename T, int V>
-__device__ __forceinline__ void gn_columns(const gn_args& A, int64_t b, int c0, int have, gn_cols<V>& K) {
-  gn_param<T, V>(A.w, A.p_type, c0, have, 1.f, K.w);
-  gn_param<T, V>(A.b, A.p_type, c0, have, 0.f, K.b);
+__device__ __forceinline__ void gn_columns(const gn_args& A, int64_t b, int c0, const row_piece<T, V>& C, gn_cols<V>& K) {
+  gn_param<T, V>(A.w, A.p_type, c0, C, 1.f, K.w);
+  gn_param<T, V>(A.b, A.p_type, c0, C, 0.f, K.b);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
-    const int64_t g = b * A.G + min(c0 + e, A.C - 1) / A.Cg;
+    const int64_t g = b * A.G + A.by_cg.div(min(c0 + e, A.C - 1));
     K.mu[e] = A.mean[g];
     K.rs[e] = A.rstd[g];
+    K.a[e] = K.rs[e] * K.w[e];
   }
 }
 // sums of dz and dz h over positions r0, r0 + step, .. < r1
 template <typename T, int V>
-__device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, const T* gp, int have, int r0, int r1, int step, const gn_cols<V>& K,
-                                                float (&sz)[V], float (&sh)[V]) {
+__device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, const T* gp, const row_piece<T, V>& C, int r0, int r1, int step,
+                                                const gn_cols<V>& K, float (&sz)[V], float (&sh)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) sz[e] = sh[e] = 0.f;
-#pragma unroll 2
-  for (int r = r0; r < r1; r += step) {
-    float v[V], d[V];
-    gn_load<T, V>(xp + (int64_t)r * A.xl, have, v);
-    gn_load<T, V>(gp + (int64_t)r * A.gl, have, d);
+  int r = r0;
+  auto rows = [&](auto count) {
+    constexpr int U = decltype(count)::value;
+    typename row_piece<T, V>::raw rx[U], rg[U];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float h = (v[e] - K.mu[e]) * K.rs[e];
-      const float dz = d[e] * gn_slope(__builtin_fmaf(h, K.w[e], K.b[e]), A.act);
-      sz[e] += dz;
-      sh[e] = __builtin_fmaf(dz, h, sh[e]);
+    for (int u = 0; u < U; ++u) {
+      rx[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
+      rg[u] = C.fetch(gp + (int64_t)(r + u * step) * A.gl);
     }
-  }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[V], d[V];
+      C.expand(rx[u], v);
+      C.expand(rg[u], d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float xm = v[e] - K.mu[e];
+        const float dz = d[e] * gn_slope(__builtin_fmaf(xm, K.a[e], K.b[e]), A.act);
+        sz[e] += dz;
+        sh[e] = __builtin_fmaf(dz, xm, sh[e]);
+      }
+    }
+    r += U * step;
+  };
+  while (r + step < r1) rows(std::integral_constant<int, 2>());
+  while (r < r1) rows(std::integral_constant<int, 1>());
+#pragma unroll
+  for (int e = 0; e < V; ++e) sh[e] *= K.rs[e];
 }
 // dx of those positions; s1, s2: of each channel's group, divided by m
 template <typename T, int V>
-__device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const T* gp, T* dp, int have, int r0, int r1, int step, const gn_cols<V>& K,
-                                           const float (&s1)[V], const float (&s2)[V]) {
-#pragma unroll 2
-  for (int r = r0; r < r1; r += step) {
-    float v[V], d[V];
-    gn_load<T, V>(xp + (int64_t)r * A.xl, have, v);
-    gn_load<T, V>(gp + (int64_t)r * A.gl, have, d);
+__device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const T* gp, T* dp, const row_piece<T, V>& C, int r0, int r1, int step,
+                                           const gn_cols<V>& K, const float (&s1)[V], const float (&s2)[V]) {
+  float k1[V], k2[V];                                                  // dx = dz a - rs s1 - (x - mu) rs^2 s2
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float h = (v[e] - K.mu[e]) * K.rs[e];
-      const float t = d[e] * gn_slope(__builtin_fmaf(h, K.w[e], K.b[e]), A.act) * K.w[e];
-      v[e] = K.rs[e] * (t - __builtin_fmaf(h, s2[e], s1[e]));
-    }
-    gn_store<T, V>(dp + (int64_t)r * A.yl, have, v);
+  for (int e = 0; e < V; ++e) {
+    k1[e] = -K.rs[e] * s1[e];
+    k2[e] = -K.rs[e] * K.rs[e] * s2[e];
   }
+  int r = r0;
+  auto rows = [&](auto count) {
+    constexpr int U = decltype(count)::value;
+    typename row_piece<T, V>::raw rx[U], rg[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      rx[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
+      rg[u] = C.fetch(gp + (int64_t)(r + u * step) * A.gl);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float v[V], d[V];
+      C.expand(rx[u], v);
+      C.expand(rg[u], d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float xm = v[e] - K.mu[e];
+        const float dz = d[e] * gn_slope(__builtin_fmaf(xm, K.a[e], K.b[e]), A.act);
+        v[e] = __builtin_fmaf(dz, K.a[e], __builtin_fmaf(xm, k2[e], k1[e]));
+      }
+      C.store(dp + (int64_t)(r + u * step) * A.yl, v, A.past);
+    }
+    r += U * step;
+  };
+  while (r + step < r1) rows(std::integral_constant<int, 2>());
+  while (r < r1) rows(std::integral_constant<int, 1>());
 }
 
 // a block a sample window, block x of grid_b taking every grid_b-th sample: part[x][0: dz, 1: dz h][C] holds the sums over its samples
 template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
-  __shared__ float cz[GN_THREADS * V], ch[GN_THREADS * V];             // [rp][W]; WIDE: s1, s2 of a thread
+  __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];   // [rp][nvec V]; WIDE: s1, s2 of a thread
   __shared__ float g1[GN_THREADS], g2[GN_THREADS];
-  const int64_t x = blockIdx.x / A.nw;
-  const gn_place P = gn_where(A, x, (int)(blockIdx.x - x * A.nw), 0);
+  const int64_t x = A.by_nw.div(blockIdx.x);
+  const gn_place P = gn_where(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
   float* out = A.part ? A.part + x * 2 * A.C + P.c0 : nullptr;
   float tz[V], th[V];
@@ -554,25 +723,27 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       const int have = P.on ? P.W - P.j * V : 0;
       if (have > 0) {
         float sz[V], sh[V];
-        gn_columns<T, V>(A, b, P.c0 + P.j * V, have, K);
-        gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, have, P.ri, A.L, A.rp, K, sz, sh);
+        const row_piece<T, V> C(have, P.W < V);
+        gn_columns<T, V>(A, b, P.c0 + P.j * V, C, K);
+        gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, C, P.ri, A.L, A.rp, K, sz, sh);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           tz[e] += sz[e];
           th[e] += sh[e];
-          if (e < have) {
-            cz[P.ri * P.W + P.j * V + e] = sz[e] * K.w[e];
-            ch[P.ri * P.W + P.j * V + e] = sh[e] * K.w[e];
-          }
+          sz[e] *= K.w[e];
+          sh[e] *= K.w[e];
         }
+        gn_lds_put<V>(cz + (P.ri * A.nvec + P.j) * V, sz);
+        gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, sh);
       }
     } else {
       float s1 = 0.f, s2 = 0.f;
       for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
         const int have = P.W - j * V;
         float sz[V], sh[V];
-        gn_columns<T, V>(A, b, P.c0 + j * V, have, K);
-        gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, have, 0, A.L, 1, K, sz, sh);
+        const row_piece<T, V> C(have, false);
+        gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
+        gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, C, 0, A.L, 1, K, sz, sh);
 #pragma unroll
         for (int e = 0; e < V; ++e)
           if (e < have) {
@@ -594,15 +765,17 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       for (int q0 = 0; q0 < P.groups; q0 += per) {
         const int g = q0 + threadIdx.x / lanes;
         const bool live = g < P.groups;
-        const int entries = live ? (WIDE ? GN_THREADS : A.rp * A.Cg) : 0;
         float s1 = 0.f, s2 = 0.f;
-        for (int t = lane; t < entries; t += lanes) {
-          const int ri = WIDE ? 0 : t / A.Cg, at = WIDE ? t : ri * P.W + g * A.Cg + (t - ri * A.Cg);
-          s1 += cz[at];
-          s2 += ch[at];
+        if (live) {
+          for (int ri = 0; ri < (WIDE ? 1 : A.rp); ++ri)
+            for (int c = lane; c < (WIDE ? GN_THREADS : A.Cg); c += lanes) {
+              const int at = WIDE ? c : ri * A.nvec * V + g * A.Cg + c;
+              s1 += cz[at];
+              s2 += ch[at];
+            }
         }
-        s1 = gn_team_sum(s1, lanes);
-        s2 = gn_team_sum(s2, lanes);
+        s1 = row_team_sum(s1, lanes);
+        s2 = row_team_sum(s2, lanes);
         if (live && lane == 0) {
           g1[g] = s1 * inv;
           g2[g] = s2 * inv;
@@ -613,32 +786,31 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
         const int have = WIDE || P.on ? P.W - j * V : 0;
         if (have <= 0) break;
-        if (WIDE) gn_columns<T, V>(A, b, P.c0 + j * V, have, K);
+        const row_piece<T, V> C(have, P.W < V);
+        if (WIDE) gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const int g = WIDE ? 0 : min(j * V + e, P.W - 1) / A.Cg;
+          const int g = WIDE ? 0 : (int)A.by_cg.div(min(j * V + e, P.W - 1));
           s1[e] = g1[g];
           s2[e] = g2[g];
         }
-        gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, have, WIDE ? 0 : P.ri, A.L, WIDE ? 1 : A.rp, K, s1, s2);
+        gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, C, WIDE ? 0 : P.ri, A.L, WIDE ? 1 : A.rp, K, s1, s2);
       }
     }
     __syncthreads();                                                    // cz, ch, g1, g2 are free again
   }
   if (WIDE || !out) return;
   const int have = P.on ? P.W - P.j * V : 0;
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (e < have) {
-      cz[P.ri * P.W + P.j * V + e] = tz[e];
-      ch[P.ri * P.W + P.j * V + e] = th[e];
-    }
+  if (have > 0) {
+    gn_lds_put<V>(cz + (P.ri * A.nvec + P.j) * V, tz);
+    gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, th);
+  }
   __syncthreads();
   for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {
     float a = 0.f, d = 0.f;
     for (int q = 0; q < A.rp; ++q) {
-      a += cz[q * P.W + c];
-      d += ch[q * P.W + c];
+      a += cz[q * A.nvec * V + c];
+      d += ch[q * A.nvec * V + c];
     }
     out[c] = a;
     out[A.C + c] = d;
@@ -648,11 +820,11 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
 // tiles of positions: part[b, tile][0: dz, 1: dz h][C]
 template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
-  __shared__ float cz[GN_THREADS * V], ch[GN_THREADS * V];
-  const int64_t u = blockIdx.x / A.tiles;
+  __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];
+  const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
-  const int64_t b = u / A.nw;
-  const gn_place P = gn_where(A, b, (int)(u - b * A.nw), tile);
+  const int64_t b = A.by_nw.div(u);
+  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
   const T* xp = (const T*)A.x + b * A.xb + P.c0;
   const T* gp = (const T*)A.dy + b * A.gb + P.c0;
@@ -662,8 +834,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   if constexpr (WIDE) {
     for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
       const int have = P.W - j * V;
-      gn_columns<T, V>(A, b, P.c0 + j * V, have, K);
-      gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, have, r0, r1, 1, K, sz, sh);
+      const row_piece<T, V> C(have, false);
+      gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
+      gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, C, r0, r1, 1, K, sz, sh);
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (e < have) {
@@ -674,21 +847,18 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   } else {
     const int have = P.on ? P.W - P.j * V : 0;
     if (have > 0) {
-      gn_columns<T, V>(A, b, P.c0 + P.j * V, have, K);
-      gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, have, r0 + P.ri, r1, A.rp, K, sz, sh);
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (e < have) {
-          cz[P.ri * P.W + P.j * V + e] = sz[e];
-          ch[P.ri * P.W + P.j * V + e] = sh[e];
-        }
+      const row_piece<T, V> C(have, P.W < V);
+      gn_columns<T, V>(A, b, P.c0 + P.j * V, C, K);
+      gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, C, r0 + P.ri, r1, A.rp, K, sz, sh);
+      gn_lds_put<V>(cz + (P.ri * A.nvec + P.j) * V, sz);
+      gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, sh);
     }
     __syncthreads();
     for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {
       float a = 0.f, d = 0.f;
       for (int q = 0; q < A.rp; ++q) {
-        a += cz[q * P.W + c];
-        d += ch[q * P.W + c];
+        a += cz[q * A.nvec * V + c];
+        d += ch[q * A.nvec * V + c];
       }
       out[c] = a;
       out[A.C + c] = d;
@@ -709,13 +879,13 @@ __global__ void __launch_bounds__(1024) k_gn_fold(gn_args A, int64_t groups, int
     const float* p = A.part + b * A.tiles * 2 * A.C + (int64_t)g * A.Cg;
     for (int i = tid; i < A.tiles * A.Cg; i += 1024) {
       const int t = i / A.Cg, c = i - t * A.Cg;
-      float w[1];
-      gn_param<T, 1>(A.w, A.p_type, g * A.Cg + c, 1, 1.f, w);
-      s1 += p[(int64_t)t * 2 * A.C + c] * w[0];
-      s2 += p[(int64_t)t * 2 * A.C + A.C + c] * w[0];
+      const int cc = g * A.Cg + c;
+      const float w = !A.w ? 1.f : A.p_type == OGL_F32 ? ((const float*)A.w)[cc] : (float)((const T*)A.w)[cc];
+      s1 += p[(int64_t)t * 2 * A.C + c] * w;
+      s2 += p[(int64_t)t * 2 * A.C + A.C + c] * w;
     }
-    s1 = gn_team_sum(s1, 64);
-    s2 = gn_team_sum(s2, 64);
+    s1 = row_team_sum(s1, 64);
+    s2 = row_team_sum(s2, 64);
     if ((tid & 63) == 0) {
       lds[tid >> 6] = s1;
       lds[16 + (tid >> 6)] = s2;
@@ -731,8 +901,10 @@ __global__ void __launch_bounds__(1024) k_gn_fold(gn_args A, int64_t groups, int
   const int64_t col = ((int64_t)blockIdx.x - groups) * 16 + (tid & 15);
   const int slice = tid >> 4;
   float a = 0.f;
-  if (col < 2 * (int64_t)A.C)
+  if (col < 2 * (int64_t)A.C) {
+#pragma unroll 8
     for (int64_t r = slice; r < rows; r += 64) a += A.part[r * 2 * A.C + col];
+  }
   lds[tid] = a;
   __syncthreads();
   for (int o = 32; o > 0; o >>= 1) {
@@ -751,10 +923,10 @@ __global__ void __launch_bounds__(1024) k_gn_fold(gn_args A, int64_t groups, int
 
 template <typename T, int V, bool WIDE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
-  const int64_t u = blockIdx.x / A.tiles;
+  const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
-  const int64_t b = u / A.nw;
-  const gn_place P = gn_where(A, b, (int)(u - b * A.nw), tile);
+  const int64_t b = A.by_nw.div(u);
+  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
   const T* xp = (const T*)A.x + b * A.xb + P.c0;
   const T* gp = (const T*)A.dy + b * A.gb + P.c0;
@@ -762,23 +934,24 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
   for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
+    const row_piece<T, V> C(have, P.W < V);
     gn_cols<V> K;
-    gn_columns<T, V>(A, b, P.c0 + j * V, have, K);
+    gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
     float s1[V], s2[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float* s = A.sums + (b * A.G + P.g0 + min(j * V + e, P.W - 1) / A.Cg) * 2;
+      const float* s = A.sums + (b * A.G + P.g0 + (int)A.by_cg.div(min(j * V + e, P.W - 1))) * 2;
       s1[e] = s[0];
       s2[e] = s[1];
     }
-    gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, have, r0 + (WIDE ? 0 : P.ri), r1, WIDE ? 1 : A.rp, K, s1, s2);
+    gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, C, r0 + (WIDE ? 0 : P.ri), r1, WIDE ? 1 : A.rp, K, s1, s2);
   }
 }
 
 // ================================================================ host ========================================================================
 struct gn_plan {
   bool rows, block, wide;
-  int nv;                      // rows: pieces a lane
+  int nv, r;                   // rows: pieces a lane, rows a team
   int64_t part, sums;          // floats of workspace
 };
 
@@ -786,20 +959,25 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
   gn_plan P = {};
   const int V = x_type == OGL_F32 ? 4 : 8;
   const int pieces = (int)ogl_cdiv(A.Cg, V);
+  A.by_cg = ogl_div::make((uint32_t)A.Cg);
   P.rows = A.L == 1 && pieces <= 4 * GN_THREADS;
   if (P.rows) {
-    // up to 256 pieces a group: teams inside a wave (1, 2 or 4 pieces a lane); above, the block is the team
-    P.block = pieces > 256;
-    A.lanes = P.block ? GN_THREADS : 1;
-    while (!P.block && A.lanes < 64 && A.lanes < pieces) A.lanes *= 2;
-    const int per = (int)ogl_cdiv(pieces, A.lanes);
-    P.nv = per <= 1 ? 1 : per <= 2 ? 2 : 4;
-    const int teams = GN_THREADS / A.lanes;
-    A.tg = 1;
-    while (A.tg < teams && A.tg < A.G) A.tg *= 2;
-    A.tr = teams / A.tg;
-    // about four blocks a CU at most: each leaves 2 C partial sums
-    A.chunks = (int)std::min<int64_t>(ogl_cdiv(A.B, A.tr), std::max<int64_t>(1, 1024 / ogl_cdiv(A.G, A.tg)));
+    // A team inside a wave: a lane for each piece up to 64, then up to 5 pieces a lane (3 in the backward of 16-bit types, for its registers).  Above
+    // that the block is the team.  Lanes that have no piece cost as much as those that do (the vector units bound these kernels), and teams of
+    // fewer lanes with more pieces each, 62500 x 600 in 30 groups: 2 lanes x 3 pieces 87 / 155 us forward / backward, 65 / 110 us so.
+    const int most = backward && V == 8 ? 3 : 5;
+    P.block = pieces > 64 * most;
+    A.lanes = P.block ? 64 : std::min(pieces, 64);
+    P.nv = (int)ogl_cdiv(pieces, P.block ? GN_THREADS : A.lanes);
+    A.tw = 64 / A.lanes;
+    A.tg = P.block ? 1 : (int)ogl_cdiv(A.G, ogl_cdiv(A.G, A.tw));      // groups of a wave: the row's, in equal shares
+    A.rpw = P.block ? 1 : std::max(1, A.tw / A.tg);
+    // several rows a team where that still leaves eight blocks a CU
+    P.r = P.nv <= 2 && !P.block && A.B * A.G * A.lanes >= 4 * 2048 * GN_THREADS ? (backward ? 2 : 4) / P.nv : 1;
+    // at most so many blocks: each leaves 2 C partial sums
+    A.chunks = (int)std::min<int64_t>(ogl_cdiv(A.B, (P.block ? 1 : 4 * A.rpw) * P.r), std::max<int64_t>(1, 1024 / ogl_cdiv(A.G, A.tg)));
+    A.by_lanes = ogl_div::make((uint32_t)A.lanes);
+    A.by_tg = ogl_div::make((uint32_t)A.tg);
     P.part = backward ? (int64_t)A.chunks * 2 * A.C : 0;
     A.by_g = ogl_div::make((uint32_t)A.G);
     return P;
@@ -828,6 +1006,9 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
   if (blocks < 1024 && A.L > A.rp * 16) tiles = std::min<int64_t>(std::min<int64_t>(ogl_cdiv(A.L, A.rp * 8), ogl_cdiv(2048, blocks)), 256);
   A.tile_rows = (int)ogl_cdiv(A.L, tiles);
   A.tiles = (int)ogl_cdiv(A.L, A.tile_rows);
+  A.by_nvec = ogl_div::make((uint32_t)A.nvec);
+  A.by_nw = ogl_div::make((uint32_t)A.nw);
+  A.by_tiles = ogl_div::make((uint32_t)A.tiles);
   A.grid_b = (int)std::min<int64_t>(A.B, std::max<int64_t>(1, 2048 / A.nw));
   if (backward) {
     P.part = (A.tiles == 1 ? (int64_t)A.grid_b : A.B * A.tiles) * 2 * A.C;
@@ -862,15 +1043,18 @@ extern "C" int64_t ogl_group_norm_workspace_bytes(int64_t B, int64_t L, int C, i
 template <typename T, int V>
 static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
   if (P.rows) {
-    const int64_t grid = ogl_cdiv(A.B * A.G, GN_THREADS / A.lanes);
+    const int64_t grid = ogl_cdiv(ogl_cdiv(A.B, P.r) * A.G, P.block ? 1 : 4 * A.tw);
     if (P.block) {
-      if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, true>), grid);
-      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, true>), grid);
-      else GN_LAUNCH((k_gn_rows_fwd<T, V, 4, true>), grid);
+      if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 1, true>), grid);
+      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 1, true>), grid);
+      else GN_LAUNCH((k_gn_rows_fwd<T, V, 4, 1, true>), grid);
     } else {
-      if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, false>), grid);
-      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, false>), grid);
-      else GN_LAUNCH((k_gn_rows_fwd<T, V, 4, false>), grid);
+      if (P.nv == 1 && P.r == 4) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 4, false>), grid);
+      else if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 1, false>), grid);
+      else if (P.nv == 2 && P.r == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 2, false>), grid);
+      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 1, false>), grid);
+      else if (P.nv == 3) GN_LAUNCH((k_gn_rows_fwd<T, V, 3, 1, false>), grid);
+      else GN_LAUNCH((k_gn_rows_fwd<T, V, 5, 1, false>), grid);
     }
     return OGL_OK;
   }
@@ -896,15 +1080,17 @@ static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, h
   if (P.rows) {
     const dim3 grid((unsigned)A.chunks, (unsigned)ogl_cdiv(A.G, A.tg));
     if (grid.y > 65535) return OGL_EINVAL;
-#define GN_ROWS(NV, BLOCK) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, BLOCK>), grid, dim3(GN_THREADS), 0, st, A)
+#define GN_ROWS(NV, R, BLOCK) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK>), grid, dim3(GN_THREADS), 0, st, A)
     if (P.block) {
-      if (P.nv == 1) GN_ROWS(1, true);
-      else if (P.nv == 2) GN_ROWS(2, true);
-      else GN_ROWS(4, true);
+      if (P.nv == 1) GN_ROWS(1, 1, true);
+      else if (P.nv == 2) GN_ROWS(2, 1, true);
+      else GN_ROWS(4, 1, true);
     } else {
-      if (P.nv == 1) GN_ROWS(1, false);
-      else if (P.nv == 2) GN_ROWS(2, false);
-      else GN_ROWS(4, false);
+      if (P.nv == 1 && P.r > 1) GN_ROWS(1, 2, false);
+      else if (P.nv == 1) GN_ROWS(1, 1, false);
+      else if (P.nv == 2) GN_ROWS(2, 1, false);
+      else if (P.nv == 3) GN_ROWS(3, 1, false);
+      else if constexpr (V == 4) GN_ROWS(5, 1, false);
     }
 #undef GN_ROWS
     rows = A.chunks;
@@ -942,6 +1128,7 @@ extern "C" int ogl_group_norm_fwd(const void* x, int64_t xb, int64_t xl, int x_t
   gn_args A = {};
   A.x = x; A.y = y; A.xb = xb; A.xl = xl; A.yb = yb; A.yl = yl; A.w = w; A.b = b; A.p_type = p_type; A.mean = mean; A.rstd = rstd;
   A.B = B; A.L = (int)L; A.C = C; A.G = G; A.Cg = C / G; A.eps = eps; A.act = act;
+  A.past = B * L * C * (x_type == OGL_F32 ? 4 : 2) >= ROW_NT_BYTES;
   const gn_plan P = gn_make(A, x_type, false);
   if (P.part > 0 && (!workspace || workspace_bytes < 4 * P.part || ((uintptr_t)workspace & 7))) return OGL_EWORKSPACE;
   A.part = (float*)workspace;
@@ -966,6 +1153,7 @@ extern "C" int ogl_group_norm_bwd(const void* dy, int64_t gb, int64_t gl, const 
   A.x = x; A.dy = dy; A.y = dx; A.xb = xb; A.xl = xl; A.gb = gb; A.gl = gl; A.yb = db_; A.yl = dl; A.w = w; A.b = b; A.p_type = p_type;
   A.mean = (float*)mean; A.rstd = (float*)rstd; A.write_dx = dx != nullptr;
   A.B = B; A.L = (int)L; A.C = C; A.G = G; A.Cg = C / G; A.act = act;
+  A.past = B * L * C * (x_type == OGL_F32 ? 4 : 2) >= ROW_NT_BYTES;
   const gn_plan P = gn_make(A, x_type, true);
   if (!workspace || workspace_bytes < 4 * (P.part + P.sums) || ((uintptr_t)workspace & 7)) return OGL_EWORKSPACE;
   A.part = (float*)workspace;

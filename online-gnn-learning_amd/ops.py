@@ -7,6 +7,8 @@ the CPU or through ATen kernels except trivial reshapes / scalar reads.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+import math
 import os
 import weakref
 
@@ -3273,20 +3275,19 @@ def cross_entropy(logits, labels, reduction="mean"):
 # --------------------------------------------------------------------------------------------
 _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ROW_FORMATS = {"int8": (torch.int8, 0), "e4m3": (torch.float8_e4m3fn, 1)}
+_ROW_CODES = {dt: code for dt, code in _ROW_FORMATS.values()}
 
 
-def _row_device(what, *tensors):
-    """The one GPU that all of ``tensors`` (None: left out) live on; work is enqueued on THAT device's current stream."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
+def _row_device(what, first, *others):
+    """The one GPU that all of the tensors (None: left out) live on; work is enqueued on THAT device's current stream."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            if first.is_cuda and t.is_cuda:
+                raise ValueError("%s: tensors on %s and %s" % (what, dev, t.device))
             raise RuntimeError("%s: ogl_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback" % what)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError("%s: tensors on %s and %s" % (what, dev, t.device))
+    if not first.is_cuda:
+        raise RuntimeError("%s: ogl_amd ops run on the GPU only (got a CPU tensor); there is no CPU fallback" % what)
     return dev
 
 
@@ -3318,7 +3319,9 @@ def _row_ids(what, ids, dev):
 
 def _row_empty(rows, cols, dtype, device):
     """[rows, cols] view of an allocation with ``padded_ld`` columns (``empty_mat`` for any row type)."""
-    return torch.empty((rows, padded_ld(cols)), dtype=dtype, device=device)[:, :cols]
+    ld = padded_ld(cols)
+    t = torch.empty((rows, ld), dtype=dtype, device=device)
+    return t if ld == cols else t[:, :cols]
 
 
 class QuantRows:
@@ -3327,12 +3330,12 @@ class QuantRows:
     A value is ``code * scale``.  ``quant_rows`` allocates one, ``quant_rows_write`` fills rows, ``quant_rows_read`` gathers them back and
     ``linear_int8`` multiplies them as they are kept (int8, one scale a row)."""
 
-    __slots__ = ("codes", "scales", "width", "group", "format")
+    __slots__ = ("codes", "scales", "width", "group", "format", "n", "ld")
 
     def __init__(self, codes, scales, width, group=None):
         width = int(width)
         group = width if group is None else min(int(group), width)
-        formats = {dt: code for dt, code in _ROW_FORMATS.values()}
+        formats = _ROW_CODES
         if codes.dim() != 2 or codes.dtype not in formats or not codes.is_contiguous() or codes.shape[1] % 64:
             raise ValueError("QuantRows: codes must be contiguous int8 or float8_e4m3fn rows of a multiple of 64 bytes")
         if not 1 <= width <= codes.shape[1]:
@@ -3346,10 +3349,11 @@ class QuantRows:
         if codes.numel() and codes.data_ptr() % 64:
             raise ValueError("QuantRows: codes must be 64-byte aligned")
         self.codes, self.scales, self.width, self.group, self.format = codes, scales, width, group, formats[codes.dtype]
+        self.n, self.ld = codes.shape
 
     @property
     def shape(self):
-        return (self.codes.shape[0], self.width)
+        return (self.n, self.width)
 
     @property
     def device(self):
@@ -3381,7 +3385,7 @@ def quant_rows_write(cache, x, slots=None, start=0):
     what = "quant_rows_write"
     x = _row_mat(what, x)
     dev = _row_device(what, cache.codes, x, slots)
-    m, n = x.shape[0], cache.shape[0]
+    m, n = x.shape[0], cache.n
     if x.shape[1] != cache.width:
         raise ValueError("%s: rows of %d columns into a cache of %d" % (what, x.shape[1], cache.width))
     start = int(start)
@@ -3395,10 +3399,10 @@ def quant_rows_write(cache, x, slots=None, start=0):
     if m == 0 or n == 0:
         return cache
     h = _lib.lib()
-    nb = h.ogl_quant_rows_workspace_bytes(m, n, slots is not None)
+    nb = 0 if slots is None else h.ogl_quant_rows_workspace_bytes(m, n, 1)
     ws = torch.empty(nb // 4, dtype=torch.int32, device=dev) if nb else None
     _row_launch(dev, "ogl_quant_rows_write", h.ogl_quant_rows_write, _ptr(x), _ld(x), _ROW_TYPES[x.dtype], m, cache.width, _ptr(slots), start,
-                _ptr(cache.codes), cache.codes.shape[1], cache.format, _ptr(cache.scales), n, cache.group, _ptr(ws), nb,
+                _ptr(cache.codes), cache.ld, cache.format, _ptr(cache.scales), n, cache.group, _ptr(ws), nb,
                 meta=dict(m=m, width=cache.width))
     return cache
 
@@ -3409,11 +3413,11 @@ def quant_rows_read(cache, rows=None, dtype=torch.float32):
     if dtype not in _ROW_TYPES:
         raise ValueError("%s: float32, bfloat16 or float16 values, not %s" % (what, dtype))
     dev = _row_device(what, cache.codes, rows)
-    m = cache.shape[0] if rows is None else _row_ids(what, rows, dev).numel()
+    m = cache.n if rows is None else _row_ids(what, rows, dev).numel()
     out = _row_empty(m, cache.width, dtype, dev)
     if m:
-        _row_launch(dev, "ogl_quant_rows_read", _lib.lib().ogl_quant_rows_read, _ptr(cache.codes), cache.codes.shape[1], cache.format,
-                    _ptr(cache.scales), cache.shape[0], cache.width, cache.group, _ptr(rows), m, _ptr(out), out.stride(0), _ROW_TYPES[dtype],
+        _row_launch(dev, "ogl_quant_rows_read", _lib.lib().ogl_quant_rows_read, _ptr(cache.codes), cache.ld, cache.format,
+                    _ptr(cache.scales), cache.n, cache.width, cache.group, _ptr(rows), m, _ptr(out), out.stride(0), _ROW_TYPES[dtype],
                     meta=dict(m=m, width=cache.width))
     return out
 
@@ -3448,7 +3452,7 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
             raise ValueError("%s: x_rows selects rows of a QuantRows" % what)
         x = quantize_rows(x)
     _row_int8(what, x)
-    N, K = w.shape
+    N, K = w.n, w.width
     if x.width != K:
         raise ValueError("%s: rows of %d columns, a weight of %d" % (what, x.width, K))
     if K >= 131072:
@@ -3456,15 +3460,15 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
     if bias is not None and (bias.dim() != 1 or bias.numel() != N or bias.dtype != torch.float32):
         raise ValueError("%s: the bias must be float32 [%d]" % (what, N))
     dev = _row_device(what, x.codes, w.codes, bias, x_rows)
-    M = x.shape[0] if x_rows is None else _row_ids(what, x_rows, dev).numel()
+    M = x.n if x_rows is None else _row_ids(what, x_rows, dev).numel()
     y = _row_empty(M, N, dtype, dev)
     if M == 0 or N == 0:
         return y
-    if x.shape[0] == 0:
+    if x.n == 0:
         raise ValueError("%s: rows of an empty table" % what)
     b = bias.contiguous() if bias is not None else None
-    _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, _ptr(x.codes), x.codes.shape[1], _ptr(x.scales), _ptr(x_rows), x.shape[0], M, K,
-                _ptr(w.codes), w.codes.shape[1], _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), y.stride(0), _ROW_TYPES[dtype],
+    _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, _ptr(x.codes), x.ld, _ptr(x.scales), _ptr(x_rows), x.n, M, K,
+                _ptr(w.codes), w.ld, _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), y.stride(0), _ROW_TYPES[dtype],
                 meta=dict(M=M, N=N, K=K))
     return y
 
@@ -3476,12 +3480,20 @@ ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def _norm_view(x):
-    """``x`` [B, *spatial, C] as [B, L, C] whose channels are contiguous and whose rows do not overlap (copied if they do)."""
-    B, C = x.shape[0], x.shape[-1]
-    v = x.reshape(B, x[0, ..., 0].numel() if B else 0, C) if x.dim() > 2 else x.unsqueeze(1)
+    """(tensor, stride of a sample, stride of a position) of ``x`` [B, *spatial, C] as [B, L, C] with contiguous channels and rows that do not overlap
+    (a copy where it has none)."""
+    C = x.shape[-1]
+    if x.dim() == 2:
+        sb, sc = x.stride()
+        if (C > 1 and sc != 1) or (x.shape[0] > 1 and sb < C):
+            x = x.contiguous()
+            sb = C
+        return x, sb, C
+    B = x.shape[0]
+    v = x.reshape(B, math.prod(x.shape[1:-1]), C)
     if (C > 1 and v.stride(2) != 1) or (v.shape[1] > 1 and v.stride(1) < C) or (B > 1 and v.stride(0) < C):
         v = v.contiguous()
-    return v
+    return v, v.stride(0), v.stride(1)
 
 
 def _norm_empty(x):
@@ -3489,60 +3501,75 @@ def _norm_empty(x):
     return _row_empty(x.shape[0], x.shape[1], x.dtype, x.device) if x.dim() == 2 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
+@functools.lru_cache(maxsize=256)
+def _norm_workspace(B, L, C, G, x_type, backward):
+    return _lib.lib().ogl_group_norm_workspace_bytes(B, L, C, G, x_type, backward)
+
+
 def group_norm_fwd(x, num_groups, weight, bias, eps, act, want_stats):
-    """(y, mean, rstd) of ``ogl_group_norm_fwd`` (statistics None unless wanted); see ``group_norm``."""
-    v = _norm_view(x)
-    (B, L, C), G = v.shape, num_groups
+    """(y, stats) of ``ogl_group_norm_fwd``, see ``group_norm``; stats: the float32 means and 1 / deviations [2, B, G], None unless wanted."""
+    B, C, G = x.shape[0], x.shape[-1], num_groups
+    L = 1 if x.dim() == 2 else math.prod(x.shape[1:-1])
     y = _norm_empty(x)
-    mean = rstd = None
-    if want_stats:
-        mean, rstd = torch.empty((2, B, G), dtype=torch.float32, device=x.device)
+    stats = torch.empty((2, B, G), dtype=torch.float32, device=x.device) if want_stats else None
     if B and L:
-        yv = _norm_view(y)
-        h, t = _lib.lib(), _ROW_TYPES[x.dtype]
-        p = weight if weight is not None else bias
-        nb = h.ogl_group_norm_workspace_bytes(B, L, C, G, t, 0)
+        x, xb, xl = _norm_view(x)
+        yb, yl = (y.stride(0), C) if y.dim() == 2 else (L * C, C)
+        t, p = _ROW_TYPES[x.dtype], weight if weight is not None else bias
+        nb = _norm_workspace(B, L, C, G, t, 0)
         ws = torch.empty(nb // 4, dtype=torch.float32, device=x.device) if nb > 0 else None
-        _row_launch(x.device, "ogl_group_norm_fwd", h.ogl_group_norm_fwd, _ptr(v), v.stride(0), v.stride(1), t, B, L, C, G, _ptr(weight), _ptr(bias),
-                    0 if p is None else _ROW_TYPES[p.dtype], eps, act, _ptr(y), yv.stride(0), yv.stride(1), _ptr(mean), _ptr(rstd), _ptr(ws), max(nb, 0),
-                    meta=dict(B=B, L=L, C=C, G=G))
-    return y, mean, rstd
+        mean = stats.data_ptr() if want_stats else None
+        _row_launch(x.device, "ogl_group_norm_fwd", _lib.lib().ogl_group_norm_fwd, x.data_ptr(), xb, xl, t, B, L, C, G, _ptr(weight), _ptr(bias),
+                    0 if p is None else _ROW_TYPES[p.dtype], eps, act, y.data_ptr(), yb, yl, mean, mean + 4 * B * G if want_stats else None, _ptr(ws),
+                    max(nb, 0), meta=dict(B=B, L=L, C=C, G=G))
+    return y, stats
 
 
-def group_norm_bwd(dy, x, num_groups, weight, bias, mean, rstd, act, want_dx=True, want_dw=True, want_db=True):
+def group_norm_bwd(dy, x, num_groups, weight, bias, stats, act, want_dx=True, want_dw=True, want_db=True):
     """(dx, dw, db) of ``ogl_group_norm_bwd``; None where not wanted."""
-    v, g = _norm_view(x), _norm_view(dy)
-    (B, L, C), G = v.shape, num_groups
+    B, C, G = x.shape[0], x.shape[-1], num_groups
+    L = 1 if x.dim() == 2 else math.prod(x.shape[1:-1])
     p = weight if weight is not None else bias
     dx = _norm_empty(x) if want_dx else None
     dw = torch.empty(C, dtype=p.dtype, device=x.device) if want_dw else None
     db = torch.empty(C, dtype=p.dtype, device=x.device) if want_db else None
     if B == 0 or L == 0:
         return dx, dw.zero_() if want_dw else None, db.zero_() if want_db else None
-    dv = _norm_view(dx) if want_dx else v
-    h, t = _lib.lib(), _ROW_TYPES[x.dtype]
-    nb = h.ogl_group_norm_workspace_bytes(B, L, C, G, t, 1)
-    ws = torch.empty(max(nb, 8) // 4, dtype=torch.float32, device=x.device)
-    _row_launch(x.device, "ogl_group_norm_bwd", h.ogl_group_norm_bwd, _ptr(g), g.stride(0), g.stride(1), _ptr(v), v.stride(0), v.stride(1), t, B, L, C, G,
-                _ptr(weight), _ptr(bias), 0 if p is None else _ROW_TYPES[p.dtype], act, _ptr(mean), _ptr(rstd), _ptr(dx), dv.stride(0), dv.stride(1),
-                _ptr(dw), _ptr(db), _ptr(ws), ws.numel() * 4, meta=dict(B=B, L=L, C=C, G=G))
+    x, xb, xl = _norm_view(x)
+    dy, gb, gl = _norm_view(dy)
+    yb, yl = (dx.stride(0), C) if want_dx and dx.dim() == 2 else (L * C, C)
+    t = _ROW_TYPES[x.dtype]
+    nb = max(_norm_workspace(B, L, C, G, t, 1), 8)
+    ws = torch.empty(nb // 4, dtype=torch.float32, device=x.device)
+    mean = stats.data_ptr()
+    _row_launch(x.device, "ogl_group_norm_bwd", _lib.lib().ogl_group_norm_bwd, dy.data_ptr(), gb, gl, x.data_ptr(), xb, xl, t, B, L, C, G, _ptr(weight),
+                _ptr(bias), 0 if p is None else _ROW_TYPES[p.dtype], act, mean, mean + 4 * B * G, _ptr(dx), yb, yl, _ptr(dw), _ptr(db), ws.data_ptr(), nb,
+                meta=dict(B=B, L=L, C=C, G=G))
     return dx, dw, db
 
 
 class _GroupNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, num_groups, eps, act):
-        y, mean, rstd = group_norm_fwd(x, num_groups, weight, bias, eps, act, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        y, stats = group_norm_fwd(x, num_groups, weight, bias, eps, act, True)
+        ctx.save_for_backward(x, weight, bias, stats)
         ctx.num_groups, ctx.act = num_groups, act
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*group_norm_bwd(dy, x, ctx.num_groups, weight, bias, mean, rstd, ctx.act, need[0], need[1], need[2]), None, None, None)
+        # (create_graph: the gradients come marked so that differentiating THEM raises; the wrapper costs, so it is left out otherwise)
+        return _group_norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _group_norm_backward(ctx, dy)
+
+
+def _group_norm_backward(ctx, dy):
+    x, weight, bias, stats = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx, dw, db = group_norm_bwd(dy, x, ctx.num_groups, weight, bias, stats, ctx.act, need[0], need[1], need[2])
+    return dx, dw, db, None, None, None
+
+
+_group_norm_backward_once = torch.autograd.function.once_differentiable(_group_norm_backward)
 
 
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):

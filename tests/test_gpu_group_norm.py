@@ -220,8 +220,8 @@ def test_captured(ops, shape, G):
     w, b = torch.ones(shape[-1], device="cuda"), torch.zeros(shape[-1], device="cuda")
 
     def body():
-        y, mean, rstd = ops.group_norm_fwd(x, G, w, b, 1e-5, 2, True)
-        return (y, *ops.group_norm_bwd(dy, x, G, w, b, mean, rstd, 2))
+        y, stats = ops.group_norm_fwd(x, G, w, b, 1e-5, 2, True)
+        return (y, *ops.group_norm_bwd(dy, x, G, w, b, stats, 2))
     body()
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
