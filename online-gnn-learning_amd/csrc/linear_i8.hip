@@ -1,8 +1,8 @@
 // Products of rows kept in 8 bits (gfx950):  y[m, n] = act((sx[m] sw[n]) * sum_k x[m, k] w[n, k] + bias[n]),  x and w int8 with one float32 scale a row.
 //
-// The sum is exact (int32 accumulators of v_mfma_i32_16x16x64_i8; |sum| <= 128^2 K < 2^31 for K < 131072, whatever
-// the bytes hold), so its order is free: waves may split K and partial sums may be joined in any order with the same result.  Rounded to float32: the
-// sum once (above 2^24), sx sw, their product, and the addition of the bias.
+// The sum is exact (int32 accumulators of v_mfma_i32_32x32x32_i8 and 16x16x64; |sum| <= 128^2 K < 2^31 for K < 131072, whatever the bytes hold), so its
+// order is free: waves may split K and partial sums may be joined in any order with the same result.  Rounded to float32: the sum once (above 2^24),
+// sx sw, their product, and the addition of the bias.
 //
 // Both operands lie K-contiguous (a weight's rows are its output channels), which is what the matrix instruction reads: 16 bytes of one row a lane.
 // Rows are a multiple of 64 bytes with zeros behind the last column, so there is no tail in K beyond a missing half step.  The weight rows are the
@@ -11,6 +11,8 @@
 #include "row_types.h"
 
 typedef int v4i32 __attribute__((ext_vector_type(4)));
+typedef int v16i32 __attribute__((ext_vector_type(16)));
+typedef int i8_piece __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes of y, wherever they lie
 typedef const __attribute__((address_space(1))) void* i8_gptr;
 typedef __attribute__((address_space(3))) void* i8_lptr;
 
@@ -37,15 +39,33 @@ __device__ __forceinline__ int64_t i8_row(const i8_args& A, int64_t m, bool& ok)
   return ok ? r : 0;
 }
 
-// 4 consecutive outputs of a row from n on
-template <typename T>
-__device__ __forceinline__ void i8_out(const i8_args& A, int64_t m, int n, v4i32 acc, float sx, const float (&sw)[4], const float (&b)[4]) {
-  float v[4];
+// scales and bias of 4 columns (behind the last one: anything)
+__device__ __forceinline__ void i8_columns(const i8_args& A, int n, float (&sw)[4], float (&b)[4]) {
+  if (n + 4 <= A.N) {
+    __builtin_memcpy(sw, A.sw + n, 16);
+    if (A.bias) __builtin_memcpy(b, A.bias + n, 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int nn = min(n + i, A.N - 1);
+      sw[i] = A.sw[nn];
+      if (A.bias) b[i] = A.bias[nn];
+    }
+  }
+  if (!A.bias) b[0] = b[1] = b[2] = b[3] = 0.f;
+}
+// 4 outputs of a row
+__device__ __forceinline__ void i8_values(const i8_args& A, v4i32 acc, float sx, const float (&sw)[4], const float (&b)[4], float (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = (float)acc[i] * (sx * sw[i]) + b[i];
     if (A.relu) v[i] = v[i] < 0.f ? 0.f : v[i];                     // (a NaN stays)
   }
+}
+template <typename T>
+__device__ __forceinline__ void i8_out(const i8_args& A, int64_t m, int n, v4i32 acc, float sx, const float (&sw)[4], const float (&b)[4]) {
+  float v[4];
+  i8_values(A, acc, sx, sw, b, v);
   T* yp = (T*)A.y + m * A.ldy + n;
   if (n + 4 <= A.N) {
     row_store<T, 4>(yp, v);
@@ -96,12 +116,7 @@ __global__ void __launch_bounds__(512) k_i8_few(i8_args A) {
     const int n = n0 + c * 4;
     if (m < A.M && n < A.N) {
       float sw[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int nn = min(n + i, A.N - 1);
-        sw[i] = A.sw[nn];
-        b[i] = A.bias ? A.bias[nn] : 0.f;
-      }
+      i8_columns(A, n, sw, b);
       bool ok;
       const int64_t row = i8_row(A, m, ok);
       i8_out<T>(A, m, n, s, ok ? A.sx[row] : 0.f, sw, b);
@@ -110,128 +125,248 @@ __global__ void __launch_bounds__(512) k_i8_few(i8_args A) {
 }
 
 // ---- many rows: BM x BN tiles through LDS ---------------------------------------------------------------------------------------------------------
-// A stage holds 128 bytes of each row, moved by LDS-DMA (16 bytes a lane, 8 lanes a row: whole 128-byte lines).  16-byte piece p of row r holds the
-// row's bytes 16 (p ^ ((r >> 1) & 7)): the 16 rows a fragment load reads side by side then touch every bank once.
-#define I8_BK 128
-
+// A stage holds 64 bytes of each row, moved by LDS-DMA (16 bytes a lane, 4 lanes a row); four stages are a ring.  16-byte piece p of row r holds the
+// row's bytes 16 (p ^ ((r >> 2) & 3)): the 16 rows a fragment load reads side by side then touch every bank once.
+// A block stays on its CU and takes every blocks-th tile.  Its steps are one sequence over all its tiles, so the first ones of the next tile are on
+// their way while the last ones of a tile multiply.
 template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m, int tiles_n) {
+__global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m, int tiles_n, int blocks) {
   constexpr int THREADS = WM * WN * 64;
-  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;                 // 16 x 16 tiles of a wave
-  constexpr int NA = BM * 8 / THREADS, NB = BN * 8 / THREADS;
-  __shared__ __align__(128) signed char sx0[BM * I8_BK], sx1[BM * I8_BK], sw0[BN * I8_BK], sw1[BN * I8_BK];
+  constexpr int TM = BM / WM / 32, TN = BN / WN / 32;                 // 32 x 32 tiles of a wave
+  constexpr int NA = BM * 4 / THREADS, NB = BN * 4 / THREADS;
+  constexpr bool PAST = BM * BN >= 65536;
+  constexpr int LINE = TN * 32 * (int)sizeof(T), UNITS = LINE / 16;    // a wave's run of columns: bytes, 16-byte units
+  constexpr int ROWS = LINE * 32 <= 4096 - 512 ? 32 : LINE * 16 <= 4096 - 512 ? 16 : 8;   // rows that are turned over at a time
+  constexpr int WAVE_LDS = ROWS * LINE + TN * 32 * 8;
+  // (arrays of their own: the compiler then knows which stage a DMA writes, and a read of another one waits for none)
+  __shared__ __align__(128) signed char x0[BM * 64], x1[BM * 64], x2[BM * 64], x3[BM * 64], w0[BN * 64], w1[BN * 64], w2[BN * 64], w3[BN * 64];
+  __shared__ __align__(128) signed char turned[WM * WN * WAVE_LDS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
+  const int tiles = tiles_m * tiles_n, steps = A.K64;
 
-  // tiles by XCD: consecutive blocks go to different XCDs, each of which takes a contiguous run of tiles, 8 row tiles wide, so that its L2 holds them
-  const int tiles = tiles_m * tiles_n;
-  const int per = tiles / 8, rest = tiles % 8, xcd = blockIdx.x % 8, nth = blockIdx.x / 8;
-  const int lin = xcd * per + min(xcd, rest) + nth;
-  const int group = lin / (8 * tiles_n), in = lin - group * 8 * tiles_n;
-  const int wide = min(8, tiles_m - group * 8);
-  const int64_t m0 = (int64_t)(group * 8 + in % wide) * BM;
-  const int n0 = in / wide * BN;
+  // Tiles by XCD: consecutive blocks run on different XCDs.  Each XCD has a contiguous run of tiles, 8 row tiles wide, so that its L2 holds what its
+  // CUs read at a time.
+  auto place = [&](int t, int64_t& m0, int& n0) {
+    const int per = tiles / 8, rest = tiles % 8, xcd = t % 8, nth = t / 8;
+    const int lin = xcd * per + min(xcd, rest) + nth;
+    const int group = lin / (8 * tiles_n), in = lin - group * 8 * tiles_n;
+    const int wide = min(8, tiles_m - group * 8);
+    m0 = (int64_t)(group * 8 + in % wide) * BM;
+    n0 = in / wide * BN;
+  };
 
-  // where this thread's pieces come from: its lane's byte inside a step (the same for all its rows: they lie 16 apart or more) and the rows' offsets
-  // in units of 64 bytes (32 bits reach 256 GB)
+  // what is fetched next: step fk of tile ft (behind the last tile: the last one again, so that every step fetches the same number of pieces).  A
+  // thread's pieces: its lane's bytes inside a step (the same for all its rows: they lie 16 apart or more) and the rows' offsets in units of 64 bytes
+  // (32 bits reach 256 GB)
+  int ft = blockIdx.x, fk = 0;
   uint32_t xrow[NA], wrow[NB];
-  const int piece = (tid & 7) ^ ((tid >> 4) & 7);
-  const signed char *xl = A.x + piece * 16, *wl = A.w + piece * 16;
+  const int piece = ((tid & 3) ^ ((tid >> 4) & 3)) * 16;
+  const signed char *xk = A.x + piece, *wk = A.w + piece;
+  auto aim = [&]() {
+    int64_t m0;
+    int n0;
+    place(ft, m0, n0);
 #pragma unroll
-  for (int u = 0; u < NA; ++u) {
-    bool ok;
-    xrow[u] = (uint32_t)((uint64_t)i8_row(A, min(m0 + ((u * THREADS + tid) >> 3), A.M - 1), ok) * (uint64_t)(A.ldx >> 6));
-  }
+    for (int u = 0; u < NA; ++u) {
+      bool ok;
+      xrow[u] = (uint32_t)((uint64_t)i8_row(A, min(m0 + ((u * THREADS + tid) >> 2), A.M - 1), ok) * (uint64_t)(A.ldx >> 6));
+    }
 #pragma unroll
-  for (int u = 0; u < NB; ++u) wrow[u] = (uint32_t)min(n0 + ((u * THREADS + tid) >> 3), A.N - 1) * (uint32_t)(A.ldw >> 6);
-  const int steps = (A.K64 + 1) >> 1;
-  const bool half = A.K64 & 1;                                        // the last step has 64 bytes only: its second half is read from the first again
-  auto fetch = [&](int k, signed char* dx, signed char* dw) {
-    const int64_t off = (int64_t)k * I8_BK - (half && k == steps - 1 && (piece & 4) ? 64 : 0);
-    const signed char *xk = xl + off, *wk = wl + off;
-#pragma unroll
-    for (int u = 0; u < NA; ++u)
-      __builtin_amdgcn_global_load_lds((i8_gptr)(xk + (uint64_t)xrow[u] * 64u), (i8_lptr)(dx + (u * THREADS + wave * 64) * 16), 16, 0, 0);
-#pragma unroll
-    for (int u = 0; u < NB; ++u)
-      __builtin_amdgcn_global_load_lds((i8_gptr)(wk + (uint64_t)wrow[u] * 64u), (i8_lptr)(dw + (u * THREADS + wave * 64) * 16), 16, 0, 0);
+    for (int u = 0; u < NB; ++u) wrow[u] = (uint32_t)min(n0 + ((u * THREADS + tid) >> 2), A.N - 1) * (uint32_t)(A.ldw >> 6);
   };
-  const int r = lane & 15, c = lane >> 4;
-  const int sw = (r >> 1) & 7;                                        // (tiles start at multiples of 16 rows: the swizzle is the lane's)
-  const int xoff = (wm * TM * 16 + r) * I8_BK, woff = (wn * TN * 16 + r) * I8_BK;
-  const int p0 = ((c ^ sw) * 16), p1 = (((4 + c) ^ sw) * 16);
+  auto advance = [&]() {
+    if (++fk == steps) {
+      fk = 0;
+      if (ft + blocks < tiles) ft += blocks;
+      aim();
+    }
+  };
+  auto fetch = [&](int u, signed char* dx, signed char* dw) {          // piece u of NA + NB
+    const uint64_t off = (uint64_t)fk * 64u;
+    if (u < NA)
+      __builtin_amdgcn_global_load_lds((i8_gptr)(xk + off + (uint64_t)xrow[u < NA ? u : 0] * 64u), (i8_lptr)(dx + (u * THREADS + wave * 64) * 16), 16, 0, 0);
+    else
+      __builtin_amdgcn_global_load_lds((i8_gptr)(wk + off + (uint64_t)wrow[u < NA ? 0 : u - NA] * 64u), (i8_lptr)(dw + ((u - NA) * THREADS + wave * 64) * 16),
+                                       16, 0, 0);
+  };
+  const int r = lane & 31, c = lane >> 5;
+  const int swz = (r >> 2) & 3;                                       // (tiles start at multiples of 32 rows: the swizzle is the lane's)
+  const int xoff = (wm * TM * 32 + r) * 64, woff = (wn * TN * 32 + r) * 64;
 
-  v4i32 acc[TN][TM];
+  v16i32 acc[TN][TM];
+  auto clear = [&]() {
 #pragma unroll
-  for (int a = 0; a < TN; ++a)
+    for (int a = 0; a < TN; ++a)
 #pragma unroll
-    for (int b = 0; b < TM; ++b) acc[a][b] = v4i32{0, 0, 0, 0};
+      for (int b = 0; b < TM; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[a][b][i] = 0;
+  };
   v4i32 fw[2][TN], fx[2][TM];
-  auto read = [&](int h, const signed char* bx, const signed char* bw, int p) {
-#pragma unroll
-    for (int a = 0; a < TN; ++a) fw[h][a] = *(const v4i32*)(bw + woff + a * 16 * I8_BK + p);
-#pragma unroll
-    for (int b = 0; b < TM; ++b) fx[h][b] = *(const v4i32*)(bx + xoff + b * 16 * I8_BK + p);
+  auto read = [&](int s, int i, const signed char* bx, const signed char* bw) {        // of the 32 bytes s of a stage the i-th fragment, 16 bytes a lane,
+    const int p = ((2 * s + c) ^ swz) * 16;                                            // in the order that the products take them
+    if (i == 0 || (i > 1 && i <= TN)) {
+      const int a = i == 0 ? 0 : i - 1;
+      fw[s][a] = *(const v4i32*)(bw + woff + a * 32 * 64 + p);
+    } else {
+      const int b = i == 1 ? 0 : i - TN;
+      fx[s][b] = *(const v4i32*)(bx + xoff + b * 32 * 64 + p);
+    }
   };
-  auto multiply = [&](int h) {
-#pragma unroll
-    for (int b = 0; b < TM; ++b)
-#pragma unroll
-      for (int a = 0; a < TN; ++a) acc[a][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][a], fx[h][b], acc[a][b], 0, 0, 0);
+  auto multiply = [&](int s, int i) {                                                  // the i-th of the wave's TM TN tiles
+    acc[i % TN][i / TN] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][i % TN], fx[s][i / TN], acc[i % TN][i / TN], 0, 0, 0);
   };
-  // one step: the fragments of its first half are in registers (0); its second half (1) is read while they multiply, then every wave is done with
-  // the stage and the next one has landed: it is refilled for the step after next while the next stage's first half is read.  (The waits are
-  // builtins: the compiler then knows that the stage it reads has landed, and waits for no younger DMA.)
-  auto step = [&](int k, signed char* cx, signed char* cw, const signed char* nx, const signed char* nw) {
-    __builtin_amdgcn_s_waitcnt(0xC07F);                               // lgkmcnt(0): the first half, read during the last multiplication
-    read(1, cx, cw, p1);
-    multiply(0);
-    __builtin_amdgcn_sched_barrier(0);
-    __builtin_amdgcn_s_waitcnt(0x0070);                               // vmcnt(0) lgkmcnt(0)
+  // A lane holds one row of y for each b, and of each 32 columns the quads 8 q + 4 c .. + 3.  Stored from there an instruction would write 32 bytes of
+  // each of 32 rows: each wave turns its rows over in LDS, ROWS at a time, and stores whole runs of columns (62500 x 600 float32: 89 us without, 73 us
+  // so).  PAST: the tiles of large products are stored past the caches, whose write-back of 33 MB or more otherwise meets the next tiles' reads (62500 x
+  // 600 float32 75 -> 67 us; 4096 x 4096 bfloat16, K = 512 20.9 -> 18.4 us; 8192 x 8192, K = 4096 293 -> 276 us).
+  // Scales and bias are loaded before the first store: a load behind it would wait for it (one counter for both, in order).
+  signed char* turn = turned + wave * WAVE_LDS;
+  auto finish = [&](int t) {
+    constexpr int E = 16 / (int)sizeof(T);
+    int64_t m0;
+    int n0;
+    place(t, m0, n0);
+    m0 += wm * TM * 32;
+    n0 += wn * TN * 32;
+    float* cols = (float*)(turn + ROWS * LINE);                        // [TN 32] scales, [TN 32] biases
+    float sx[TM], sw = 0.f, bias = 0.f;
+    if (lane < TN * 32) {
+      const int n = min(n0 + lane, A.N - 1);
+      sw = A.sw[n];
+      if (A.bias) bias = A.bias[n];
+    }
+#pragma unroll
+    for (int b = 0; b < TM; ++b) {
+      bool ok;
+      const int64_t row = i8_row(A, min(m0 + b * 32 + r, A.M - 1), ok);
+      sx[b] = ok ? A.sx[row] : 0.f;
+    }
+    if (lane < TN * 32) {
+      cols[lane] = sw;
+      cols[TN * 32 + lane] = bias;
+    }
+    __builtin_amdgcn_wave_barrier();
+    const bool full = m0 + TM * 32 <= A.M && n0 + TN * 32 <= A.N;
+#pragma unroll
+    for (int b = 0; b < TM; ++b) {
+      float v[TN * 4][4];
+#pragma unroll
+      for (int u = 0; u < TN * 4; ++u) {
+        const int at = u * 8 + c * 4;
+        float w[4], d[4];
+        *(float4*)w = *(const float4*)(cols + at);
+        *(float4*)d = *(const float4*)(cols + TN * 32 + at);
+        const v16i32& s = acc[u >> 2][b];
+        const int q = (u & 3) * 4;
+        i8_values(A, v4i32{s[q], s[q + 1], s[q + 2], s[q + 3]}, sx[b], w, d, v[u]);
+      }
+#pragma unroll
+      for (int h = 0; h < 32 / ROWS; ++h) {
+        const int rr = r & (ROWS - 1);
+        if (ROWS == 32 || r / ROWS == h) {
+#pragma unroll
+          for (int u = 0; u < TN * 4; ++u) {
+            const int at = (u * 8 + c * 4) * (int)sizeof(T);
+            row_store<T, 4>((T*)(turn + rr * LINE + ((at >> 4) ^ (rr & (UNITS - 1))) * 16 + (at & 15)), v[u]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < ROWS * UNITS / 64; ++it) {
+          const int line = it * (64 / UNITS) + lane / UNITS, unit = lane % UNITS;
+          const int64_t m = m0 + b * 32 + h * ROWS + line;
+          const int n = n0 + unit * E;
+          const T* from = (const T*)(turn + line * LINE + (unit ^ (line & (UNITS - 1))) * 16);
+          T* yp = (T*)A.y + m * A.ldy + n;
+          if (full) {
+            if constexpr (PAST) __builtin_nontemporal_store(*(const i8_piece*)from, (i8_piece*)yp);
+            else __builtin_memcpy(yp, from, 16);
+          } else if (m < A.M && n < A.N) {
+            if (n + E <= A.N) {
+              __builtin_memcpy(yp, from, 16);
+            } else {
+              for (int i = 0; i < E; ++i)
+                if (n + i < A.N) yp[i] = from[i];
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // One step: the fragments of a stage's first 32 bytes are in registers; those of its second 32 are read while the first multiply.  Then every wave
+  // has read the stage, and the next one (fetched three steps ago; two younger ones may be on their way) has landed: its first fragments are read, and
+  // the stage is refilled for four steps on, while the second ones multiply.  Reads and fetches go between the products one by one: issued in one go,
+  // those of all waves queue for the LDS and hold up the products behind them.  (The waits are builtins: the compiler then waits for no younger DMA.)
+  constexpr int PIECES = NA + NB, TILES = TM * TN, FRAGS = TM + TN, SLOTS = TILES > FRAGS ? TILES : FRAGS;
+  auto step = [&](signed char* cx, signed char* cw, const signed char* nx, const signed char* nw) {
+#pragma unroll
+    for (int i = 0; i < SLOTS; ++i) {
+      if (i < TILES) multiply(0, i);
+      if (i < FRAGS) read(1, i, cx, cw);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __builtin_amdgcn_s_waitcnt((2 * PIECES & 15) | (2 * PIECES >> 4 << 14) | 0x0070);   // vmcnt(2 PIECES) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if (k + 2 < steps) fetch(k + 2, cx, cw);
-    read(0, nx, nw, p0);                                              // (behind the last step: an old stage, never multiplied)
-    if (!(half && k == steps - 1)) multiply(1);
+#pragma unroll
+    for (int i = 0; i < (SLOTS > PIECES ? SLOTS : PIECES); ++i) {
+      if (i < TILES) multiply(1, i);
+      if (i < FRAGS) read(0, i, nx, nw);                              // (behind the last step: a stage that is never multiplied)
+      if (i < PIECES) fetch(i, cx, cw);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    advance();
   };
-  fetch(0, sx0, sw0);
-  __builtin_amdgcn_s_waitcnt(0x0070);
+  aim();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+#pragma unroll
+    for (int u = 0; u < PIECES; ++u) fetch(u, q == 0 ? x0 : q == 1 ? x1 : q == 2 ? x2 : x3, q == 0 ? w0 : q == 1 ? w1 : q == 2 ? w2 : w3);
+    advance();
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);                                 // (all of them: no path into the loop then has a stage on its way)
   __builtin_amdgcn_s_barrier();
-  if (steps > 1) fetch(1, sx1, sw1);
-  read(0, sx0, sw0, p0);
-  for (int k = 0; k < steps; k += 2) {
-    step(k, sx0, sw0, sx1, sw1);
-    if (k + 1 < steps) step(k + 1, sx1, sw1, sx0, sw0);
-  }
-
 #pragma unroll
-  for (int a = 0; a < TN; ++a) {
-    const int n = n0 + (wn * TN + a) * 16 + c * 4;
-    if (n >= A.N) continue;
-    float s[4], b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int nn = min(n + i, A.N - 1);
-      s[i] = A.sw[nn];
-      b[i] = A.bias ? A.bias[nn] : 0.f;
+  for (int i = 0; i < FRAGS; ++i) read(0, i, x0, w0);
+  int at = 0;                                                          // the stage that the sequence of steps has come to
+  for (int t = blockIdx.x; t < tiles; t += blocks) {
+    clear();
+    for (int k = 0;;) {
+      if (at == 0) {
+        step(x0, w0, x1, w1);
+        at = 1;
+        if (++k == steps) break;
+      }
+      if (at == 1) {
+        step(x1, w1, x2, w2);
+        at = 2;
+        if (++k == steps) break;
+      }
+      if (at == 2) {
+        step(x2, w2, x3, w3);
+        at = 3;
+        if (++k == steps) break;
+      }
+      step(x3, w3, x0, w0);
+      at = 0;
+      if (++k == steps) break;
     }
-#pragma unroll
-    for (int t = 0; t < TM; ++t) {
-      const int64_t m = m0 + (wm * TM + t) * 16 + r;
-      if (m >= A.M) continue;
-      bool ok;
-      const int64_t row = i8_row(A, m, ok);
-      i8_out<T>(A, m, n, acc[a][t], ok ? A.sx[row] : 0.f, s, b);
-    }
+    finish(t);
   }
+  __builtin_amdgcn_s_waitcnt(0x0070);                                 // what was fetched behind the last step
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int BM, int BN, int WM, int WN>
-static int i8_launch_tile(const i8_args& A, hipStream_t st) {
+static int i8_launch_tile(const i8_args& A, int blocks, hipStream_t st) {
   const int64_t tm = ogl_cdiv(A.M, BM), tn = ogl_cdiv(A.N, BN);
-  if (tm * tn * WM * WN * 64 > UINT32_MAX || tm * tn > INT32_MAX) return OGL_EINVAL;
-  hipLaunchKernelGGL((k_i8_tile<T, BM, BN, WM, WN>), dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), 0, st, A, (int)tm, (int)tn);
+  if (tm * tn > INT32_MAX) return OGL_EINVAL;
+  blocks = (int)std::min<int64_t>(tm * tn, blocks);
+  hipLaunchKernelGGL((k_i8_tile<T, BM, BN, WM, WN>), dim3((unsigned)blocks), dim3(WM * WN * 64), 0, st, A, (int)tm, (int)tn, blocks);
   return OGL_OK;
 }
 
@@ -246,8 +381,8 @@ static int i8_launch(const i8_args& A, hipStream_t st) {
     hipLaunchKernelGGL((k_i8_few<T, 4>), dim3(nb, 1), dim3(512), 0, st, A);
     return OGL_OK;
   }
-  if (ogl_cdiv(A.M, 256) * ogl_cdiv(A.N, 256) >= 256) return i8_launch_tile<T, 256, 256, 2, 4>(A, st);
-  return i8_launch_tile<T, 64, 64, 2, 2>(A, st);
+  if (ogl_cdiv(A.M, 256) * ogl_cdiv(A.N, 256) >= 256) return i8_launch_tile<T, 256, 256, 2, 4>(A, 256, st);   // a block a CU
+  return i8_launch_tile<T, 64, 64, 2, 2>(A, 768, st);
 }
 
 extern "C" int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const int64_t* rows, int64_t nrows, int64_t M, int K, const void* w, int64_t ldw,
