@@ -381,7 +381,12 @@ static int i8_launch(const i8_args& A, hipStream_t st) {
     hipLaunchKernelGGL((k_i8_few<T, 4>), dim3(nb, 1), dim3(512), 0, st, A);
     return OGL_OK;
   }
-  if (ogl_cdiv(A.M, 256) * ogl_cdiv(A.N, 256) >= 256) return i8_launch_tile<T, 256, 256, 2, 4>(A, 256, st);   // a block a CU
+  // Large tiles read each operand less often, small ones fill the card.  256 x 256 (one block a CU) from a tile a CU on: 4096 x 4096, K = 4096 70 us,
+  // in 128 x 128 tiles 101 us, in 64 x 64 ones 145 us.  128 x 128 (two blocks a CU) from 3 tiles for 4 CUs on, 1024 x 4096, K = 4096: 26 us, 64 x 64
+  // 39 us, 256 x 256 46 us; 512 x 4096 (128 tiles) 22.6 us, 64 x 64 21.2 us; with few steps the epilogue weighs more, 16000 x 600, K = 602 (625 tiles):
+  // 25 us, 64 x 64 23 us.
+  if (ogl_cdiv(A.M, 256) * ogl_cdiv(A.N, 256) >= 256) return i8_launch_tile<T, 256, 256, 2, 4>(A, 256, st);
+  if (ogl_cdiv(A.M, 128) * ogl_cdiv(A.N, 128) >= 192 && A.K64 >= 16) return i8_launch_tile<T, 128, 128, 2, 2>(A, 512, st);
   return i8_launch_tile<T, 64, 64, 2, 2>(A, 768, st);
 }
 
