@@ -61,6 +61,7 @@ class SnapshotGraph:
         target = torch.as_tensor(np.asarray(target)).reshape(n, -1)[:, :1].to(torch.int64)
         self.target_table = target.to(self.device).contiguous()
         self.edata = {}
+        self._quantized = {}
         self.n_present = 0
         self.cut = 0
         self.ndata = {"feat": self.feat_table[:0], "target": self.target_table[:0]}
@@ -78,6 +79,7 @@ class SnapshotGraph:
         g.handle = ops.GraphHandle(g._indptr, g._indices, g._keys)
         g.feat_table, g.target_table = other.feat_table, other.target_table
         g.edata = {}
+        g._quantized = other._quantized
         g.n_present = g.cut = 0
         g.ndata = {"feat": g.feat_table[:0], "target": g.target_table[:0]}
         return g
@@ -86,6 +88,21 @@ class SnapshotGraph:
         self.handle.set_snapshot(n_present, cut)
         self.n_present, self.cut = int(n_present), int(cut)
         self.ndata = {"feat": self.feat_table[:self.n_present], "target": self.target_table[:self.n_present]}
+
+    def quantized_features(self):
+        """The present vertices' feature rows in 8 bits (``ops.QuantRows``, int8, one scale a row).  Each row is quantised once, when a call first
+        finds it present: features are static, so the cache only grows with the stream (shared by the views of one stream)."""
+        q = self._quantized
+        if "rows" not in q:
+            q["rows"], q["written"] = ops.quant_rows(self.n_total, self.feat_table.shape[1], device=self.device), 0
+        rows, done = q["rows"], q["written"]
+        if done < self.n_present:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("quantized_features: rows %d .. %d are new, call it once before the capture" % (done, self.n_present))
+            ops.quant_rows_write(rows, self.feat_table[done:self.n_present], start=done)
+            q["written"] = self.n_present
+        n = self.n_present
+        return ops.QuantRows(rows.codes[:n], rows.scales[:n], rows.width)
 
     def number_of_nodes(self):
         return self.n_present

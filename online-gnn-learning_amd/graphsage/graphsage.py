@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from .sageconv import SAGEConv
+from .sageconv import SAGEConv, read_back
 
 
 INREPO_T_IMAGES = True   # in-repo pooling layers: W^T images prepared with the step's others
@@ -16,7 +16,8 @@ INREPO_T_IMAGES = True   # in-repo pooling layers: W^T images prepared with the 
 
 class GraphSAGE(nn.Module):
     def __init__(self, in_feats, n_hidden, n_classes, n_layers, activation, dropout, aggregator_type, edge_feats=None,
-                 pool_feats=None):
+                 pool_feats=None, norm=None):
+        # norm (optional): width -> the hidden layers' norm, a callable on their rows (``lambda width: GroupNorm(g, width)``)
         super().__init__()
         # the live reference layer (DGL SAGEConv) takes neither edge_feats nor pool_feats (graphsage_dgl.py:41
         # comments them out); the in-repo layer does, so they are forwarded for its modes only
@@ -24,9 +25,11 @@ class GraphSAGE(nn.Module):
         if aggregator_type != "pool":
             extra = dict(edge_feats=edge_feats, pool_feats=pool_feats)
         self.layers = nn.ModuleList()
-        self.layers.append(SAGEConv(in_feats, n_hidden, aggregator_type, feat_drop=dropout, activation=activation, **extra))
+        self.layers.append(SAGEConv(in_feats, n_hidden, aggregator_type, feat_drop=dropout, activation=activation,
+                                    norm=norm(n_hidden) if norm else None, **extra))
         for _ in range(n_layers - 1):
-            self.layers.append(SAGEConv(n_hidden, n_hidden, aggregator_type, feat_drop=dropout, activation=activation, **extra))
+            self.layers.append(SAGEConv(n_hidden, n_hidden, aggregator_type, feat_drop=dropout, activation=activation,
+                                        norm=norm(n_hidden) if norm else None, **extra))
         self.layers.append(SAGEConv(n_hidden, n_classes, aggregator_type, feat_drop=dropout, activation=None, **extra))
 
     @contextlib.contextmanager
@@ -139,6 +142,7 @@ class GraphSAGE(nn.Module):
         launch of its backward (a device-scope fence per block inside the forward launch costs 33 us at 512 seeds) — until that
         backward has run the loss tensor holds NaN.  The default writes the value in the forward launch: a loss that is only
         logged, guarded or evaluated is always valid."""
+        x = read_back(x)
         if torch.is_grad_enabled() and ops.get_gemm_mode() != "f32" and ops.PREPARE_WEIGHT_IMAGES:
             self._prepare_step_images(blocks, x)
         h = x
@@ -160,6 +164,7 @@ class GraphSAGE(nn.Module):
         return ops.cross_entropy(logits, labels, "mean"), None, logits
 
     def forward(self, blocks, x):
+        x = read_back(x)
         if torch.is_grad_enabled() and ops.get_gemm_mode() != "f32" and ops.PREPARE_WEIGHT_IMAGES:
             self._prepare_step_images(blocks, x)
         h = x

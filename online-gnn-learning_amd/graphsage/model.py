@@ -393,6 +393,9 @@ class HipSupervisedGraphSage(SupervisedGraphSage):
     # (0 = one launch sequence per batch of batch_full seeds, as the reference's loop).  131 072 rows x 608 floats = 320 MB per
     # intermediate: the products run as several rounds of tiles instead of a fraction of one
     FUSE_INFERENCE_ROWS = 131072
+    # the per-pass tables from features kept in 8 bits (SnapshotGraph.quantized_features) and weights quantised for the pass: about 0.4 % of a
+    # row's largest feature off, at 8-bit matrix rate (opt-in: float32 tables otherwise)
+    quantize_features = False
 
     def _projection_tables(self, graph, layer0):
         """(P0, S0) of ``SAGEConv.project_tables`` for every present vertex, once per pass (weights are fixed during it).
@@ -401,7 +404,7 @@ class HipSupervisedGraphSage(SupervisedGraphSage):
         that rank: a batch takes its self term from S0 and its neighbour term from P0), written in place into its block of
         the full tables, then ONE all-gather per table exchanges the blocks: the rows outside a rank's range are the halo
         embeddings its sampled neighbourhoods reach into (on a power-law graph every batch does)."""
-        feat = graph.ndata["feat"]
+        feat = graph.quantized_features() if self.quantize_features else graph.ndata["feat"]
         dev = graph.device
 
         def project(lo, hi, blocks):

@@ -28,7 +28,8 @@ from .. import ops
 
 class GatheredRows:
     """Lazy ``table[ids]``: the row gather is fused into the consuming GEMM / reduction loaders so
-    ``graph.ndata['feat'][input_nodes]`` (R/.../pytorch/model.py:54,88,182,232) is never materialised."""
+    ``graph.ndata['feat'][input_nodes]`` (R/.../pytorch/model.py:54,88,182,232) is never materialised.  ``table`` may be rows kept in 8 bits
+    (``ops.QuantRows``): a layer then reads them back as float32 rows first."""
 
     def __init__(self, table: torch.Tensor, ids, proj: torch.Tensor = None):
         # proj (optional, inference only): the (P0, S0) pair of SAGEConv.project_tables for EVERY table row, computed
@@ -44,7 +45,16 @@ class GatheredRows:
         return GatheredRows(self.table, self.ids[:n], self.proj)
 
     def materialize(self):
+        if isinstance(self.table, ops.QuantRows):
+            return ops.quant_rows_read(self.table, self.ids)
         return ops.gather_rows(self.table, self.ids)
+
+
+def read_back(x):
+    """``x``, rows kept in 8 bits read back: what the layers' float kernels take (projected tables are kept: they are float32)."""
+    if isinstance(x, GatheredRows) and x.proj is None and isinstance(x.table, ops.QuantRows):
+        return x.materialize()
+    return x
 
 
 # inference self term S0[dst]: from this output width on it is added by the neighbour GEMM (accumulators start at the table row:
@@ -129,6 +139,7 @@ class SAGEConv(nn.Module):
         t = self._aggre_type
         if t not in ("pool", "mean", "gcn", "meanpool", "maxpool", "lstm"):
             raise KeyError("Aggregator type {} not recognized.".format(t))
+        feat = read_back(feat)
         lazy = isinstance(feat, GatheredRows)
         if self.training and self.feat_drop.p > 0:
             # feat_drop on the layer input (graphsage_dgl.py:41): one HIP launch, fused with the row gather when the input
@@ -349,13 +360,19 @@ class SAGEConv(nn.Module):
         """The per-weight-version tables consumed by _forward_cached, for ``table[rows]`` (default: every row):
         ``P0 = relu(fc_pool(x))`` and ``S0`` = the self term of the combine with every bias of it folded in
         (``fc_self(x) + b_self + b_neigh`` for 'pool', ``x . W[:, :in]^T + b`` of the concat -> fc_neigh modes).
-        ``out = (P0_rows, S0_rows)`` writes into caller-owned row blocks (a rank's slice of the exchanged tables)."""
+        ``out = (P0_rows, S0_rows)`` writes into caller-owned row blocks (a rank's slice of the exchanged tables).
+        A table of rows kept in 8 bits (``ops.QuantRows``, int8 with one scale a row) is multiplied as it is kept, the weights quantised row by
+        row for the call (inference only, like the path that reads the tables)."""
         if self.fc_pool is None:
             raise KeyError("aggregator {} has no pooling projection".format(self._aggre_type))
         if self._aggre_type == "pool":
             w_self, b_self = self.fc_self.weight, self._summed_bias()
         else:
             w_self, b_self = self.fc_neigh.weight[:, :self._in_feats], self.fc_neigh.bias
+        if isinstance(table, ops.QuantRows):
+            with torch.no_grad():
+                return (ops.linear_int8(table, ops.quantize_rows(self.fc_pool.weight), self.fc_pool.bias, True, rows, out=out[0] if out else None),
+                        ops.linear_int8(table, ops.quantize_rows(w_self), b_self, False, rows, out=out[1] if out else None))
         p0 = ops.linear_fwd(table, self.fc_pool.weight, self.fc_pool.bias, relu=True, x_rows=rows, out=out[0] if out else None)
         s0 = ops.linear_fwd(table, w_self, b_self, x_rows=rows, out=out[1] if out else None)
         return p0, s0

@@ -3437,10 +3437,11 @@ def _row_int8(what, q):
     return q
 
 
-def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
+def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32, out=None):
     """``act((sx sw^T) * (x @ w^T) + bias)`` of rows kept in int8: ``x`` a ``QuantRows`` of tokens or vertices (``x_rows``: int64 ids of the rows to
     take; ids outside it count as zero rows) or a float matrix, which is quantised row by row first; ``w`` the ``QuantRows`` of a weight
-    [out_features, in_features].  The sum is exact, the rest float32, the result ``dtype``.  Inference only: there is no gradient."""
+    [out_features, in_features].  The sum is exact, the rest float32, the result ``dtype``, written into ``out`` if that is given.  Inference
+    only: there is no gradient."""
     what = "linear_int8"
     _row_int8(what, w)
     if dtype not in _ROW_TYPES:
@@ -3461,14 +3462,21 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32):
         raise ValueError("%s: the bias must be float32 [%d]" % (what, N))
     dev = _row_device(what, x.codes, w.codes, bias, x_rows)
     M = x.n if x_rows is None else _row_ids(what, x_rows, dev).numel()
-    y = _row_empty(M, N, dtype, dev)
+    if out is None:
+        y = _row_empty(M, N, dtype, dev)
+    else:
+        y = out
+        if (tuple(y.shape) != (M, N) or y.dtype != dtype or (N > 1 and y.stride(1) != 1) or (M > 1 and y.stride(0) < N)
+                or (torch.is_grad_enabled() and y.requires_grad)):
+            raise ValueError("%s: out must be a %s matrix [%d, %d] with contiguous columns and no gradient" % (what, dtype, M, N))
+        _row_device(what, x.codes, y)
     if M == 0 or N == 0:
         return y
     if x.n == 0:
         raise ValueError("%s: rows of an empty table" % what)
     b = bias.contiguous() if bias is not None else None
     _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, _ptr(x.codes), x.ld, _ptr(x.scales), _ptr(x_rows), x.n, M, K,
-                _ptr(w.codes), w.ld, _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), y.stride(0), _ROW_TYPES[dtype],
+                _ptr(w.codes), w.ld, _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), _ld(y), _ROW_TYPES[dtype],
                 meta=dict(M=M, N=N, K=K))
     return y
 

@@ -5,7 +5,7 @@ The north star's layering is "Python host code calls PyTorch-ROCm custom ops ove
 replace, op for op, what the reference's layer reaches through DGL / ATen at
 R/train/graphsage/pytorch/graphsage_dgl.py:55-59 (``layer(block, h)`` -> sampling, ``to_block``, ``feat[input_nodes]``,
 ``copy_src``/``max``, ``nn.Linear``, ``CrossEntropyLoss``, ``Adam``).  Differentiable ops (``linear``, ``pool_max``,
-``neighbor_reduce``, ``cross_entropy``, ``dropout``) are registered as composite ops over the package's
+``neighbor_reduce``, ``cross_entropy``, ``dropout``, ``group_norm``) are registered as composite ops over the package's
 ``autograd.Function`` nodes, so ``torch.ops.ogl.linear(...)`` back-propagates through the HIP backward kernels.  There
 is no CPU kernel: a CPU tensor raises (no fallback).
 
@@ -52,6 +52,12 @@ def _define():
     D("adam_step(Tensor(a!) p, Tensor g, Tensor(b!) m, Tensor(c!) v, int step, float lr=1e-3, float beta1=0.9, "
       "float beta2=0.999, float eps=1e-8) -> ()")
     D("dropout_rows(Tensor x, float p, int seed, int ctr, Tensor? rows=None) -> Tensor")
+    # rows kept in 8 bits: codes [n, ld], scales [n, groups] as ops.QuantRows describes them, passed as their tensors
+    D("quantize_rows(Tensor x, int? group=None, str fmt='int8') -> (Tensor, Tensor)")
+    D("quant_rows_write(Tensor(a!) codes, Tensor(b!) scales, int width, int? group, Tensor x, Tensor? slots=None, int start=0) -> ()")
+    D("quant_rows_read(Tensor codes, Tensor scales, int width, int? group=None, Tensor? rows=None, ScalarType? dtype=None) -> Tensor")
+    D("linear_int8(Tensor codes, Tensor scales, Tensor w_codes, Tensor w_scales, int width, Tensor? bias=None, bool relu=False, "
+      "Tensor? x_rows=None, ScalarType? dtype=None) -> Tensor")
     # differentiable (composite over the autograd.Function nodes of ops.py)
     D("linear(Tensor x, Tensor w, Tensor? bias=None, Tensor? x2=None, Tensor? w2=None, bool relu=False, "
       "Tensor? x_rows=None, Tensor? x2_rows=None, Tensor? bias2=None) -> Tensor")
@@ -59,6 +65,7 @@ def _define():
     D("pool_max(Tensor x, Tensor w, Tensor? bias, Tensor idx, Tensor? x_rows=None) -> Tensor")
     D("cross_entropy(Tensor logits, Tensor labels, str reduction='mean') -> Tensor")
     D("dropout(Tensor x, float p, Tensor? rows=None) -> Tensor")
+    D("group_norm(Tensor x, int num_groups, Tensor? weight=None, Tensor? bias=None, float eps=1e-5, str? activation=None) -> Tensor")
 
     def cuda(name, fn):
         lib.impl(name, fn, "CUDA")
@@ -81,14 +88,30 @@ def _define():
     cuda("adam_step", lambda p, g, m, v, step, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8:
          ops.adam_step(p, g, m, v, step, lr, beta1, beta2, eps))
     cuda("dropout_rows", lambda x, p, seed, ctr, rows=None: ops.dropout_rows(x, p, seed, ctr, rows))
+    cuda("quantize_rows", lambda x, group=None, fmt="int8": _quantize_rows(x, group, fmt))
+    cuda("quant_rows_write", _quant_rows_write)
+    cuda("quant_rows_read", lambda codes, scales, width, group=None, rows=None, dtype=None:
+         ops.quant_rows_read(ops.QuantRows(codes, scales, width, group), rows, dtype or torch.float32))
+    cuda("linear_int8", lambda codes, scales, w_codes, w_scales, width, bias=None, relu=False, x_rows=None, dtype=None:
+         ops.linear_int8(ops.QuantRows(codes, scales, width), ops.QuantRows(w_codes, w_scales, width), bias, relu, x_rows, dtype or torch.float32))
     composite("linear", lambda x, w, bias=None, x2=None, w2=None, relu=False, x_rows=None, x2_rows=None, bias2=None:
               ops.linear(x, w, bias, x2, w2, relu, x_rows, x2_rows, bias2))
     composite("neighbor_reduce", ops.neighbor_reduce)
     composite("pool_max", lambda x, w, bias, idx, x_rows=None: ops.pool_max(x, w, bias, idx, x_rows))
     composite("cross_entropy", lambda logits, labels, reduction="mean": ops.cross_entropy(logits, labels, reduction))
     composite("dropout", lambda x, p, rows=None: ops.dropout(x, p, rows))
+    composite("group_norm", ops.group_norm)
     _LIB = lib
     return lib
+
+
+def _quantize_rows(x, group, fmt):
+    q = ops.quantize_rows(x, group, fmt)
+    return q.codes, q.scales
+
+
+def _quant_rows_write(codes, scales, width, group, x, slots=None, start=0):
+    ops.quant_rows_write(ops.QuantRows(codes, scales, width, group), x, slots, start)
 
 
 def _build_block(dst, picks):
