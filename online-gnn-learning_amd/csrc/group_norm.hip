@@ -95,8 +95,8 @@ __device__ __forceinline__ float gn_slope(float z, int act) {
 }
 
 // channel parameters c .. of a piece (`none` where there are none)
-template <typename T, int V>
-__device__ __forceinline__ void gn_param(const void* p, int p_type, int c, const row_piece<T, V>& P, float none, float (&v)[V]) {
+template <typename T, int V, typename PIECE>
+__device__ __forceinline__ void gn_param(const void* p, int p_type, int c, const PIECE& P, float none, float (&v)[V]) {
   if (!p) {
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = none;
@@ -382,9 +382,9 @@ __device__ __forceinline__ int gn_group_lanes(int groups) {
 }
 
 // (mean, M2) of each of the block's groups over positions r0 .. r1, handed to `done(group of the window, mean, M2)` by one lane a group.
-// NARROW: sums and squares around the channel's value at r0 (the same pivot for every thread of a channel, so they add up), a channel's mean and M2
-// from them, and the channels of a group joined around the first one's mean.
-template <typename T, int V, bool WIDE, typename F>
+// NARROW: a thread's sums and squares around its first value, from them its (mean, M2); those of a channel's threads joined around the first one's mean,
+// then those of a group's channels likewise.
+template <typename T, int V, bool WIDE, typename PIECE, typename F>
 __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place& P, int r0, int r1, gn_stats_lds& S, F done) {
   const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + (int64_t)r0 * A.xl;
   const int rows = r1 - r0;
@@ -393,44 +393,65 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
     const int have = P.on ? P.W - P.j * V : 0;
     if (have > 0) {
       float k[V], s[V], q[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] = q[e] = 0.f;
-      const row_piece<T, V> C(have, P.W < V);
-      const T* p = xp + P.j * V;
-      const typename row_piece<T, V>::raw pivot = C.fetch(p);
+      const PIECE C(have, P.W < V);
       const int64_t step = (int64_t)A.rp * A.xl;
-      p += P.ri * A.xl;
-      for (int r = P.ri; r < rows; r += 8 * A.rp, p += 8 * step) {     // eight loads in flight
-        typename row_piece<T, V>::raw raw[8];
+      const T* p = xp + P.j * V + P.ri * A.xl;
+      int r = P.ri;
+      auto take = [&](auto count, auto first) {                        // that many loads in flight
+        constexpr int U = decltype(count)::value;
+        typename PIECE::raw raw[U];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (r + u * A.rp < rows) raw[u] = C.fetch(p + u * step);
-        if (r == P.ri) C.expand(pivot, k);
+        for (int u = 0; u < U; ++u) raw[u] = C.fetch(p + u * step);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          if (r + u * A.rp >= rows) break;
+        for (int u = 0; u < U; ++u) {
           float v[V];
           C.expand(raw[u], v);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float d = v[e] - k[e];
-            s[e] += d;
-            q[e] = __builtin_fmaf(d, d, q[e]);
+            if (decltype(first)::value && u == 0) {
+              k[e] = v[e];
+              s[e] = q[e] = 0.f;
+            } else {
+              const float d = v[e] - k[e];
+              s[e] += d;
+              q[e] = __builtin_fmaf(d, d, q[e]);
+            }
           }
         }
+        r += U * A.rp;
+        p += U * step;
+      };
+      const std::integral_constant<int, 1> one;
+      const std::integral_constant<int, 8> eight;
+      if (r < rows) {
+        if (r + 7 * A.rp < rows) take(eight, std::true_type());
+        else take(one, std::true_type());
+        while (r + 7 * A.rp < rows) take(eight, std::false_type());
+        if (r + 3 * A.rp < rows) take(std::integral_constant<int, 4>(), std::false_type());
+        while (r < rows) take(one, std::false_type());
+        const float n = (float)((r - P.ri) / A.rp), by = 1.f / n;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float d = s[e] * by;
+          k[e] += d;
+          q[e] = gn_not_negative(__builtin_fmaf(-d, s[e], q[e]));
+        }
+        gn_lds_put<V>(S.a + (P.ri * A.nvec + P.j) * V, k);
+        gn_lds_put<V>(S.q + (P.ri * A.nvec + P.j) * V, q);
       }
-      gn_lds_put<V>(S.a + (P.ri * A.nvec + P.j) * V, s);
-      gn_lds_put<V>(S.q + (P.ri * A.nvec + P.j) * V, q);
     }
     __syncthreads();
     for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {               // (entry c of position 0 is this thread's from here on)
-      float s = 0.f, q = 0.f;
-      for (int ri = 0; ri < A.rp; ++ri) {
-        s += S.a[ri * A.nvec * V + c];
-        q += S.q[ri * A.nvec * V + c];
+      const float first = S.a[c];
+      float s = 0.f, q = S.q[c];
+      const int most = min(A.rp, rows), whole = rows / A.rp, rest = rows - whole * A.rp;
+      for (int ri = 1; ri < most; ++ri) {
+        const float n = (float)(whole + (ri < rest)), d = S.a[ri * A.nvec * V + c] - first;
+        s = __builtin_fmaf(n, d, s);
+        q += __builtin_fmaf(n * d, d, S.q[ri * A.nvec * V + c]);
       }
       const float d = s * in;
-      S.a[c] = (float)xp[c] + d;
+      S.a[c] = first + d;
       S.q[c] = gn_not_negative(__builtin_fmaf(-d, s, q));
     }
   } else {
@@ -440,7 +461,7 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
       const int have = P.W - j * V;
       for (int r = 0; r < rows; ++r) {
         float v[V];
-        row_piece<T, V>(have, false).load(xp + (int64_t)r * A.xl + j * V, v);
+        PIECE(have, false).load(xp + (int64_t)r * A.xl + j * V, v);
         if (n == 0) k = v[0];
 #pragma unroll
         for (int e = 0; e < V; ++e)
@@ -484,15 +505,15 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
 }
 
 // y of positions r0 .. r1 from the window's statistics, which `stats` (called once by every thread) puts into LDS while the first loads are on their way
-template <typename T, int V, bool WIDE, typename F>
+template <typename T, int V, bool WIDE, typename PIECE, typename F>
 __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& P, int r0, int r1, const float* mean, const float* rstd, F stats) {
   constexpr int U = 2;
-  typedef typename row_piece<T, V>::raw raw_t;
+  typedef typename PIECE::raw raw_t;
   const int step = WIDE ? 1 : A.rp, first = r0 + (WIDE ? 0 : P.ri);
   raw_t ahead[U];
   if constexpr (!WIDE) {
     const int have = P.on ? P.W - P.j * V : 0;
-    const row_piece<T, V> C(have, P.W < V);
+    const PIECE C(have, P.W < V);
     const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + P.j * V;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -502,12 +523,12 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
   for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
-    const row_piece<T, V> C(have, P.W < V);
+    const PIECE C(have, P.W < V);
     const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + j * V;
     T* yp = (T*)A.y + P.b * A.yb + P.c0 + j * V;
     float mu[V], a[V], bb[V];
-    gn_param<T, V>(A.w, A.p_type, P.c0 + j * V, C, 1.f, a);
-    gn_param<T, V>(A.b, A.p_type, P.c0 + j * V, C, 0.f, bb);
+    gn_param<T, V, PIECE>(A.w, A.p_type, P.c0 + j * V, C, 1.f, a);
+    gn_param<T, V, PIECE>(A.b, A.p_type, P.c0 + j * V, C, 0.f, bb);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const int g = WIDE ? 0 : (int)A.by_cg.div(min(j * V + e, P.W - 1));
@@ -535,15 +556,15 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
 }
 
 // a block a sample window
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
   __shared__ gn_stats_lds S;
   __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
   const int64_t b = A.by_nw.div(blockIdx.x);
   const gn_place P = gn_where(A, b, (int)(blockIdx.x - (uint32_t)b * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
-  gn_apply_rows<T, V, WIDE>(A, P, 0, A.L, mean, rstd, [&]() {
-    gn_block_stats<T, V, WIDE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
+  gn_apply_rows<T, V, WIDE, PIECE>(A, P, 0, A.L, mean, rstd, [&]() {
+    gn_block_stats<T, V, WIDE, PIECE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
       const float r = 1.f / sqrtf(m2 * inv + A.eps);
       mean[g] = mu;
       rstd[g] = r;
@@ -556,7 +577,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
 }
 
 // tiles of positions: part[(b, group), tile] = (mean, M2)
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_stats(gn_args A) {
   __shared__ gn_stats_lds S;
   const uint32_t u = A.by_tiles.div(blockIdx.x);
@@ -564,12 +585,12 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_stats(gn_args A) {
   const int64_t b = A.by_nw.div(u);
   const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
-  gn_block_stats<T, V, WIDE>(A, P, r0, r1, S, [&](int g, float mu, float m2) {
+  gn_block_stats<T, V, WIDE, PIECE>(A, P, r0, r1, S, [&](int g, float mu, float m2) {
     float2* o = (float2*)A.part + (b * A.G + P.g0 + g) * A.tiles + tile;
     *o = make_float2(mu, m2);
   });
 }
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_apply(gn_args A) {
   __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
   const uint32_t u = A.by_tiles.div(blockIdx.x);
@@ -577,7 +598,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_apply(gn_args A) {
   const int64_t b = A.by_nw.div(u);
   const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows;
-  gn_apply_rows<T, V, WIDE>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd, [&]() {
+  gn_apply_rows<T, V, WIDE, PIECE>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd, [&]() {
     const int lanes = gn_group_lanes(P.groups);
     const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
     const float total = (float)A.Cg * (float)A.L;
@@ -617,10 +638,10 @@ template <int V>
 struct gn_cols {
   float mu[V], rs[V], w[V], a[V], b[V];                                // a = rs w: z = (x - mu) a + b
 };
-template <typename T, int V>
-__device__ __forceinline__ void gn_columns(const gn_args& A, int64_t b, int c0, const row_piece<T, V>& C, gn_cols<V>& K) {
-  gn_param<T, V>(A.w, A.p_type, c0, C, 1.f, K.w);
-  gn_param<T, V>(A.b, A.p_type, c0, C, 0.f, K.b);
+template <typename T, int V, typename PIECE>
+__device__ __forceinline__ void gn_columns(const gn_args& A, int64_t b, int c0, const PIECE& C, gn_cols<V>& K) {
+  gn_param<T, V, PIECE>(A.w, A.p_type, c0, C, 1.f, K.w);
+  gn_param<T, V, PIECE>(A.b, A.p_type, c0, C, 0.f, K.b);
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const int64_t g = b * A.G + A.by_cg.div(min(c0 + e, A.C - 1));
@@ -630,15 +651,15 @@ __device__ __forceinline__ void gn_columns(const gn_args& A, int64_t b, int c0, 
   }
 }
 // sums of dz and dz h over positions r0, r0 + step, .. < r1
-template <typename T, int V>
-__device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, const T* gp, const row_piece<T, V>& C, int r0, int r1, int step,
+template <typename T, int V, typename PIECE>
+__device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, const T* gp, const PIECE& C, int r0, int r1, int step,
                                                 const gn_cols<V>& K, float (&sz)[V], float (&sh)[V]) {
 #pragma unroll
   for (int e = 0; e < V; ++e) sz[e] = sh[e] = 0.f;
   int r = r0;
   auto rows = [&](auto count) {
     constexpr int U = decltype(count)::value;
-    typename row_piece<T, V>::raw rx[U], rg[U];
+    typename PIECE::raw rx[U], rg[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       rx[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
@@ -665,8 +686,8 @@ __device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, c
   for (int e = 0; e < V; ++e) sh[e] *= K.rs[e];
 }
 // dx of those positions; s1, s2: of each channel's group, divided by m
-template <typename T, int V>
-__device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const T* gp, T* dp, const row_piece<T, V>& C, int r0, int r1, int step,
+template <typename T, int V, typename PIECE>
+__device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const T* gp, T* dp, const PIECE& C, int r0, int r1, int step,
                                            const gn_cols<V>& K, const float (&s1)[V], const float (&s2)[V]) {
   float k1[V], k2[V];                                                  // dx = dz a - rs s1 - (x - mu) rs^2 s2
 #pragma unroll
@@ -677,7 +698,7 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
   int r = r0;
   auto rows = [&](auto count) {
     constexpr int U = decltype(count)::value;
-    typename row_piece<T, V>::raw rx[U], rg[U];
+    typename PIECE::raw rx[U], rg[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       rx[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
@@ -703,7 +724,7 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
 }
 
 // a block a sample window, block x of grid_b taking every grid_b-th sample: part[x][0: dz, 1: dz h][C] holds the sums over its samples
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
   __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];   // [rp][nvec V]; WIDE: s1, s2 of a thread
   __shared__ float g1[GN_THREADS], g2[GN_THREADS];
@@ -723,9 +744,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       const int have = P.on ? P.W - P.j * V : 0;
       if (have > 0) {
         float sz[V], sh[V];
-        const row_piece<T, V> C(have, P.W < V);
-        gn_columns<T, V>(A, b, P.c0 + P.j * V, C, K);
-        gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, C, P.ri, A.L, A.rp, K, sz, sh);
+        const PIECE C(have, P.W < V);
+        gn_columns<T, V, PIECE>(A, b, P.c0 + P.j * V, C, K);
+        gn_channel_sums<T, V, PIECE>(A, xp + P.j * V, gp + P.j * V, C, P.ri, A.L, A.rp, K, sz, sh);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           tz[e] += sz[e];
@@ -741,9 +762,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
         const int have = P.W - j * V;
         float sz[V], sh[V];
-        const row_piece<T, V> C(have, false);
-        gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
-        gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, C, 0, A.L, 1, K, sz, sh);
+        const PIECE C(have, false);
+        gn_columns<T, V, PIECE>(A, b, P.c0 + j * V, C, K);
+        gn_channel_sums<T, V, PIECE>(A, xp + j * V, gp + j * V, C, 0, A.L, 1, K, sz, sh);
 #pragma unroll
         for (int e = 0; e < V; ++e)
           if (e < have) {
@@ -786,15 +807,15 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
         const int have = WIDE || P.on ? P.W - j * V : 0;
         if (have <= 0) break;
-        const row_piece<T, V> C(have, P.W < V);
-        if (WIDE) gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
+        const PIECE C(have, P.W < V);
+        if (WIDE) gn_columns<T, V, PIECE>(A, b, P.c0 + j * V, C, K);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           const int g = WIDE ? 0 : (int)A.by_cg.div(min(j * V + e, P.W - 1));
           s1[e] = g1[g];
           s2[e] = g2[g];
         }
-        gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, C, WIDE ? 0 : P.ri, A.L, WIDE ? 1 : A.rp, K, s1, s2);
+        gn_dx_rows<T, V, PIECE>(A, xp + j * V, gp + j * V, dp + j * V, C, WIDE ? 0 : P.ri, A.L, WIDE ? 1 : A.rp, K, s1, s2);
       }
     }
     __syncthreads();                                                    // cz, ch, g1, g2 are free again
@@ -818,7 +839,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
 }
 
 // tiles of positions: part[b, tile][0: dz, 1: dz h][C]
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];
   const uint32_t u = A.by_tiles.div(blockIdx.x);
@@ -834,9 +855,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   if constexpr (WIDE) {
     for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
       const int have = P.W - j * V;
-      const row_piece<T, V> C(have, false);
-      gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
-      gn_channel_sums<T, V>(A, xp + j * V, gp + j * V, C, r0, r1, 1, K, sz, sh);
+      const PIECE C(have, false);
+      gn_columns<T, V, PIECE>(A, b, P.c0 + j * V, C, K);
+      gn_channel_sums<T, V, PIECE>(A, xp + j * V, gp + j * V, C, r0, r1, 1, K, sz, sh);
 #pragma unroll
       for (int e = 0; e < V; ++e)
         if (e < have) {
@@ -847,9 +868,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   } else {
     const int have = P.on ? P.W - P.j * V : 0;
     if (have > 0) {
-      const row_piece<T, V> C(have, P.W < V);
-      gn_columns<T, V>(A, b, P.c0 + P.j * V, C, K);
-      gn_channel_sums<T, V>(A, xp + P.j * V, gp + P.j * V, C, r0 + P.ri, r1, A.rp, K, sz, sh);
+      const PIECE C(have, P.W < V);
+      gn_columns<T, V, PIECE>(A, b, P.c0 + P.j * V, C, K);
+      gn_channel_sums<T, V, PIECE>(A, xp + P.j * V, gp + P.j * V, C, r0 + P.ri, r1, A.rp, K, sz, sh);
       gn_lds_put<V>(cz + (P.ri * A.nvec + P.j) * V, sz);
       gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, sh);
     }
@@ -921,7 +942,7 @@ __global__ void __launch_bounds__(1024) k_gn_fold(gn_args A, int64_t groups, int
   }
 }
 
-template <typename T, int V, bool WIDE>
+template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
   const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
@@ -934,9 +955,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
   for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
-    const row_piece<T, V> C(have, P.W < V);
+    const PIECE C(have, P.W < V);
     gn_cols<V> K;
-    gn_columns<T, V>(A, b, P.c0 + j * V, C, K);
+    gn_columns<T, V, PIECE>(A, b, P.c0 + j * V, C, K);
     float s1[V], s2[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -944,13 +965,14 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
       s1[e] = s[0];
       s2[e] = s[1];
     }
-    gn_dx_rows<T, V>(A, xp + j * V, gp + j * V, dp + j * V, C, r0 + (WIDE ? 0 : P.ri), r1, WIDE ? 1 : A.rp, K, s1, s2);
+    gn_dx_rows<T, V, PIECE>(A, xp + j * V, gp + j * V, dp + j * V, C, r0 + (WIDE ? 0 : P.ri), r1, WIDE ? 1 : A.rp, K, s1, s2);
   }
 }
 
 // ================================================================ host ========================================================================
 struct gn_plan {
   bool rows, block, wide;
+  bool even;                   // maps: every window is whole pieces
   int nv, r;                   // rows: pieces a lane, rows a team
   int64_t part, sums;          // floats of workspace
 };
@@ -1000,6 +1022,7 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
   A.nw = (int)ogl_cdiv(A.G, A.gw);
   A.nvec = (int)ogl_cdiv((int64_t)A.gw * A.Cg, V);
   A.rp = P.wide ? 1 : GN_THREADS / A.nvec;
+  P.even = A.C % V == 0 && (int64_t)A.gw * A.Cg % V == 0;
   // a block a sample window where there are enough of them to fill the card or little to do in each; else tiles of 8 positions a thread or more
   const int64_t blocks = A.B * A.nw;
   int64_t tiles = 1;
@@ -1042,6 +1065,8 @@ extern "C" int64_t ogl_group_norm_workspace_bytes(int64_t B, int64_t L, int C, i
 
 template <typename T, int V>
 static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
+  typedef row_piece<T, V> cut;
+  typedef row_whole<T, V> whole;
   if (P.rows) {
     const int64_t grid = ogl_cdiv(ogl_cdiv(A.B, P.r) * A.G, P.block ? 1 : 4 * A.tw);
     if (P.block) {
@@ -1059,23 +1084,28 @@ static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
     return OGL_OK;
   }
   if (A.tiles == 1) {
-    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true>), A.B * A.nw);
-    else GN_LAUNCH((k_gn_sample_fwd<T, V, false>), A.B * A.nw);
+    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true, cut>), A.B * A.nw);
+    else if (P.even) GN_LAUNCH((k_gn_sample_fwd<T, V, false, whole>), A.B * A.nw);
+    else GN_LAUNCH((k_gn_sample_fwd<T, V, false, cut>), A.B * A.nw);
     return OGL_OK;
   }
   const int64_t grid = A.B * A.nw * A.tiles;
   if (P.wide) {
-    GN_LAUNCH((k_gn_stats<T, V, true>), grid);
-    GN_LAUNCH((k_gn_apply<T, V, true>), grid);
+    GN_LAUNCH((k_gn_stats<T, V, true, cut>), grid);
+    GN_LAUNCH((k_gn_apply<T, V, true, cut>), grid);
   } else {
-    GN_LAUNCH((k_gn_stats<T, V, false>), grid);
-    GN_LAUNCH((k_gn_apply<T, V, false>), grid);
+    if (P.even) GN_LAUNCH((k_gn_stats<T, V, false, whole>), grid);
+    else GN_LAUNCH((k_gn_stats<T, V, false, cut>), grid);
+    if (P.even) GN_LAUNCH((k_gn_apply<T, V, false, whole>), grid);
+    else GN_LAUNCH((k_gn_apply<T, V, false, cut>), grid);
   }
   return OGL_OK;
 }
 
 template <typename T, int V>
 static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, hipStream_t st) {
+  typedef row_piece<T, V> cut;
+  typedef row_whole<T, V> whole;
   int64_t rows = 0, groups = 0;
   if (P.rows) {
     const dim3 grid((unsigned)A.chunks, (unsigned)ogl_cdiv(A.G, A.tg));
@@ -1095,12 +1125,14 @@ static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, h
 #undef GN_ROWS
     rows = A.chunks;
   } else if (A.tiles == 1) {
-    if (P.wide) GN_LAUNCH((k_gn_sample_bwd<T, V, true>), (int64_t)A.grid_b * A.nw);
-    else GN_LAUNCH((k_gn_sample_bwd<T, V, false>), (int64_t)A.grid_b * A.nw);
+    if (P.wide) GN_LAUNCH((k_gn_sample_bwd<T, V, true, cut>), (int64_t)A.grid_b * A.nw);
+    else if (P.even) GN_LAUNCH((k_gn_sample_bwd<T, V, false, whole>), (int64_t)A.grid_b * A.nw);
+    else GN_LAUNCH((k_gn_sample_bwd<T, V, false, cut>), (int64_t)A.grid_b * A.nw);
     rows = A.grid_b;
   } else {
-    if (P.wide) GN_LAUNCH((k_gn_bwd_sums<T, V, true>), A.B * A.nw * A.tiles);
-    else GN_LAUNCH((k_gn_bwd_sums<T, V, false>), A.B * A.nw * A.tiles);
+    if (P.wide) GN_LAUNCH((k_gn_bwd_sums<T, V, true, cut>), A.B * A.nw * A.tiles);
+    else if (P.even) GN_LAUNCH((k_gn_bwd_sums<T, V, false, whole>), A.B * A.nw * A.tiles);
+    else GN_LAUNCH((k_gn_bwd_sums<T, V, false, cut>), A.B * A.nw * A.tiles);
     rows = A.B * A.tiles;
     groups = A.write_dx ? A.B * A.G : 0;
   }
@@ -1109,8 +1141,9 @@ static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, h
   if (groups + folds > 0)
     hipLaunchKernelGGL(k_gn_fold<T>, dim3((unsigned)(groups + folds)), dim3(1024), 0, st, A, groups, rows, dw, db);
   if (groups > 0) {
-    if (P.wide) GN_LAUNCH((k_gn_bwd_apply<T, V, true>), A.B * A.nw * A.tiles);
-    else GN_LAUNCH((k_gn_bwd_apply<T, V, false>), A.B * A.nw * A.tiles);
+    if (P.wide) GN_LAUNCH((k_gn_bwd_apply<T, V, true, cut>), A.B * A.nw * A.tiles);
+    else if (P.even) GN_LAUNCH((k_gn_bwd_apply<T, V, false, whole>), A.B * A.nw * A.tiles);
+    else GN_LAUNCH((k_gn_bwd_apply<T, V, false, cut>), A.B * A.nw * A.tiles);
   }
   return OGL_OK;
 }
@@ -1128,7 +1161,7 @@ extern "C" int ogl_group_norm_fwd(const void* x, int64_t xb, int64_t xl, int x_t
   gn_args A = {};
   A.x = x; A.y = y; A.xb = xb; A.xl = xl; A.yb = yb; A.yl = yl; A.w = w; A.b = b; A.p_type = p_type; A.mean = mean; A.rstd = rstd;
   A.B = B; A.L = (int)L; A.C = C; A.G = G; A.Cg = C / G; A.eps = eps; A.act = act;
-  A.past = B * L * C * (x_type == OGL_F32 ? 4 : 2) >= ROW_NT_BYTES;
+  A.past = (double)B * (double)L * C * (x_type == OGL_F32 ? 4 : 2) >= (double)ROW_NT_BYTES;
   const gn_plan P = gn_make(A, x_type, false);
   if (P.part > 0 && (!workspace || workspace_bytes < 4 * P.part || ((uintptr_t)workspace & 7))) return OGL_EWORKSPACE;
   A.part = (float*)workspace;
@@ -1153,7 +1186,7 @@ extern "C" int ogl_group_norm_bwd(const void* dy, int64_t gb, int64_t gl, const 
   A.x = x; A.dy = dy; A.y = dx; A.xb = xb; A.xl = xl; A.gb = gb; A.gl = gl; A.yb = db_; A.yl = dl; A.w = w; A.b = b; A.p_type = p_type;
   A.mean = (float*)mean; A.rstd = (float*)rstd; A.write_dx = dx != nullptr;
   A.B = B; A.L = (int)L; A.C = C; A.G = G; A.Cg = C / G; A.act = act;
-  A.past = B * L * C * (x_type == OGL_F32 ? 4 : 2) >= ROW_NT_BYTES;
+  A.past = (double)B * (double)L * C * (x_type == OGL_F32 ? 4 : 2) >= (double)ROW_NT_BYTES;
   const gn_plan P = gn_make(A, x_type, true);
   if (!workspace || workspace_bytes < 4 * (P.part + P.sums) || ((uintptr_t)workspace & 7)) return OGL_EWORKSPACE;
   A.part = (float*)workspace;

@@ -75,6 +75,29 @@ struct row_piece {
   }
 };
 
+// The same where every run is a multiple of V: no ends to cut, so loads in a row have nothing between them.
+template <typename T, int V>
+struct row_whole {
+  typedef typename ogl_vec<T, V>::type raw;
+  static constexpr int n = V;
+  static constexpr bool tiny = false;
+  __device__ __forceinline__ row_whole(int, bool) {}
+  __device__ __forceinline__ raw fetch(const T* __restrict__ p) const {
+    raw t;
+    __builtin_memcpy(&t, p, 16);
+    return t;
+  }
+  __device__ __forceinline__ void expand(raw t, float (&v)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)t[i];
+  }
+  __device__ __forceinline__ void load(const T* __restrict__ p, float (&v)[V]) const { expand(fetch(p), v); }
+  __device__ __forceinline__ void store(T* __restrict__ p, const float (&v)[V], bool past) const {
+    if (past) row_store_nt<T, V>(p, v);
+    else row_store<T, V>(p, v);
+  }
+};
+
 // n / d for 0 <= n < 2^31 and 1 <= d < 2^31 as a multiplication: m = ceil(2^(31 + s) / d) with 2^s >= d, so m d = 2^(31 + s) + e, e < d <= 2^s,
 // and n m / 2^(31 + s) exceeds n / d by n e / (d 2^(31 + s)) < 1 / d: the floor is the quotient.  m < 2^32.
 struct ogl_div {
