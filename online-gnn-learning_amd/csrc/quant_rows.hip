@@ -278,6 +278,28 @@ __global__ void __launch_bounds__(256) k_quant_owner_max(const int64_t* __restri
   if (s >= 0 && s < n) atomicMax(owner + s, (int32_t)i);
 }
 
+// CH codes times their scale (keep = 0: zeros, whatever was loaded)
+template <int FMT, int CH>
+__device__ __forceinline__ void qr_expand(const uint32_t (&c)[CH / 4], uint32_t keep, float s, float (&v)[CH]) {
+#pragma unroll
+  for (int d = 0; d < CH / 4; ++d) {
+    const int w = (int)(c[d] & keep);
+    if constexpr (FMT == 0) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) v[4 * d + b] = (float)(int)(signed char)(w >> (8 * b)) * s;
+    } else {
+      v[4 * d] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * s;
+      v[4 * d + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1) * s;
+      v[4 * d + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2) * s;
+      v[4 * d + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * s;
+    }
+  }
+  // The product is rounded to float32, then to the type.  Without this (it emits nothing) the compiler may make one v_fma_mixlo_f16 of both, which
+  // rounds once.
+#pragma unroll
+  for (int e = 0; e < CH; ++e) asm("" : "+v"(v[e]));
+}
+
 // Read back, rows by id or in order: 16 bytes of output a thread and store (CH columns), REP of them 256 chunks apart with their loads issued
 // together.  Every thread of the grid has chunks (ceil(width / CH) of them in a row), so narrow rows waste no lanes.
 template <typename T, int FMT, int REP>
@@ -313,19 +335,7 @@ __global__ void __launch_bounds__(256) k_dequant_rows(const unsigned char* __res
   for (int q = 0; q < REP; ++q) {
     if (at[q] >= m) continue;
     float v[CH];
-#pragma unroll
-    for (int d = 0; d < CH / 4; ++d) {
-      const int w = (int)c[q][d];
-      if constexpr (FMT == 0) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) v[4 * d + b] = (float)(int)(signed char)(w >> (8 * b)) * s[q];
-      } else {
-        v[4 * d] = __builtin_amdgcn_cvt_f32_fp8(w, 0) * s[q];
-        v[4 * d + 1] = __builtin_amdgcn_cvt_f32_fp8(w, 1) * s[q];
-        v[4 * d + 2] = __builtin_amdgcn_cvt_f32_fp8(w, 2) * s[q];
-        v[4 * d + 3] = __builtin_amdgcn_cvt_f32_fp8(w, 3) * s[q];
-      }
-    }
+    qr_expand<FMT, CH>(c[q], ~0u, s[q], v);
     T* op = out + at[q] * ldo + e0[q];
     if (e0[q] + CH <= width) {
       if (past) row_store_nt<T, CH>(op, v);
@@ -334,6 +344,62 @@ __global__ void __launch_bounds__(256) k_dequant_rows(const unsigned char* __res
 #pragma unroll
       for (int b = 0; b < CH; ++b)
         if (e0[q] + b < width) op[b] = (T)v[b];
+    }
+  }
+}
+
+// Many rows that are wide enough for a wave each: a wave takes R rows one below the other, so ids, row addresses and the scale of a whole row are
+// scalars, and a chunk costs its loads, conversions and store.
+template <typename T, int FMT, int R>
+__global__ void __launch_bounds__(256) k_dequant_wide(const unsigned char* __restrict__ codes, int64_t ldc, const float* __restrict__ scales, int64_t n,
+                                                      int width, int G, const int64_t* __restrict__ rows, int64_t m, int per_row, ogl_div per_group,
+                                                      T* __restrict__ out, int64_t ldo, bool past) {
+  constexpr int CH = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const int64_t row0 = ((int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * R;
+  if (row0 >= m) return;
+  const unsigned char* cp[R];
+  const float* sp[R];
+  uint32_t keep[R];                                                    // all ones: the row is there
+  float whole[R];
+#pragma unroll
+  for (int q = 0; q < R; ++q) {
+    const int64_t i = min(row0 + q, m - 1);
+    const int64_t r = rows ? rows[i] : i;
+    const bool ok = r >= 0 && r < n;
+    cp[q] = codes + (ok ? r : 0) * ldc;
+    sp[q] = scales + (ok ? r : 0) * G;
+    keep[q] = ok ? ~0u : 0u;
+    whole[q] = ok ? sp[q][0] : 0.f;
+  }
+  for (int chunk = lane; chunk < per_row; chunk += 64) {
+    const int e0 = chunk * CH;
+    uint32_t c[R][CH / 4];
+    float s[R];
+#pragma unroll
+    for (int q = 0; q < R; ++q) __builtin_memcpy(c[q], cp[q] + e0, CH);
+    if (G == 1) {
+#pragma unroll
+      for (int q = 0; q < R; ++q) s[q] = whole[q];
+    } else {
+      const int g = (int)per_group.div((uint32_t)chunk);
+#pragma unroll
+      for (int q = 0; q < R; ++q) s[q] = keep[q] ? sp[q][g] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < R; ++q) {
+      if (row0 + q >= m) break;
+      float v[CH];
+      qr_expand<FMT, CH>(c[q], keep[q], s[q], v);
+      T* op = out + (row0 + q) * ldo + e0;
+      if (e0 + CH <= width) {
+        if (past) row_store_nt<T, CH>(op, v);
+        else row_store<T, CH>(op, v);
+      } else {
+#pragma unroll
+        for (int b = 0; b < CH; ++b)
+          if (e0 + b < width) op[b] = (T)v[b];
+      }
     }
   }
 }
@@ -431,12 +497,19 @@ extern "C" int ogl_quant_rows_read(const void* codes, int64_t ldc, int format, c
   // chunk 204 us, 2 186 us, 4 167 us, 8 157 us; with stores past the caches 192, -, 164, 166 us and the next launch's 158 us become 124 us).
   const bool many = chunks >= 4 * 2048 * 256;
   const bool past = chunks * 16 >= ROW_NT_BYTES;
+  // A wave a row (four of them) where a row keeps half a wave busy: the same rows 166 -> 144 us (two rows 147, eight 149), 131072 rows of 1024 codes
+  // to bfloat16 75 -> 69 us.  The other form spends its time on addresses: a division, two products of 64 bits and two loads for 16 bytes.
+  const bool wide = many && per_row >= 32 && n > 0;
 #define QR_REP(T, F, R) \
   hipLaunchKernelGGL((k_dequant_rows<T, F, R>), dim3((unsigned)ogl_cdiv(chunks, 256 * (R))), dim3(256), 0, st, (const unsigned char*)codes, ldc, scales, n, \
                      width, G, rows, m, dr, dg, (T*)out, ldo, past)
+#define QR_WIDE(T, F) \
+  hipLaunchKernelGGL((k_dequant_wide<T, F, 4>), dim3((unsigned)ogl_cdiv(m, 4 * 4)), dim3(256), 0, st, (const unsigned char*)codes, ldc, scales, n, \
+                     width, G, rows, m, per_row, dg, (T*)out, ldo, past)
 #define QR_READ(T, F) \
   do { \
-    if (many) QR_REP(T, F, 4); \
+    if (wide) QR_WIDE(T, F); \
+    else if (many) QR_REP(T, F, 4); \
     else QR_REP(T, F, 1); \
   } while (0)
   if (format == OGL_ROWS_INT8) {
@@ -449,6 +522,7 @@ extern "C" int ogl_quant_rows_read(const void* codes, int64_t ldc, int format, c
     else QR_READ(ogl_f16, 1);
   }
 #undef QR_READ
+#undef QR_WIDE
 #undef QR_REP
   OGL_CHECK_LAUNCH();
   return OGL_OK;

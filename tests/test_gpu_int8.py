@@ -164,6 +164,26 @@ def test_strided_rows_and_ranges(ops):
     assert (ops.quant_rows_read(empty, torch.tensor([0, 1], device="cuda")) == 0).all()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("w,group", [(602, None), (1031, 128), (270, 8), (100, None)])
+def test_many_rows_read(ops, fmt, dtype, w, group):
+    """Enough rows for every form of the reading kernel: the product in float32, rounded once more to the type; ids outside the cache are zero rows."""
+    n, m = 5000, 4 * 2048 * 256 * 8 // w + 3
+    gen = torch.Generator(device="cuda").manual_seed(w)
+    cache = ops.quantize_rows(torch.randn(n, w, device="cuda", generator=gen), group, fmt)
+    rows = torch.randint(-3, n + 3, (m,), device="cuda", generator=gen)
+    rows[0], rows[-1] = 2 ** 40, -2 ** 40
+    got = ops.quant_rows_read(cache, rows, dtype)
+    ok = ((rows >= 0) & (rows < n)).unsqueeze(1)
+    at = rows.clamp(0, n - 1)
+    at = torch.where(ok[:, 0], at, torch.zeros_like(at))
+    scales = torch.repeat_interleave(cache.scales, cache.group, dim=1)[:, :w]
+    want = torch.where(ok, cache.codes[:, :w].float()[at] * scales[at], torch.zeros((), device="cuda")).to(dtype)
+    assert torch.equal(got, want)
+    assert not torch.signbit(got[~ok[:, 0]]).any()
+
+
 def test_rows_behind_four_gigabytes(ops):
     """Row offsets that pass 32 bits."""
     n, w = 4_300_000, 1000                                                           # 4.4 GB of codes
