@@ -135,9 +135,12 @@ __global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m
   constexpr int TM = BM / WM / 32, TN = BN / WN / 32;                 // 32 x 32 tiles of a wave
   constexpr int NA = BM * 4 / THREADS, NB = BN * 4 / THREADS;
   constexpr bool PAST = BM * BN >= 65536;
-  constexpr int LINE = TN * 32 * (int)sizeof(T), UNITS = LINE / 16;    // a wave's run of columns: bytes, 16-byte units
-  constexpr int ROWS = LINE * 32 <= 4096 - 512 ? 32 : LINE * 16 <= 4096 - 512 ? 16 : 8;   // rows that are turned over at a time
-  constexpr int WAVE_LDS = ROWS * LINE + TN * 32 * 8;
+  // what a wave turns over at a time: AT of its tiles side by side (128 bytes of a row, or what there is of them), ROWS rows
+  constexpr int AT = TN * 32 * (int)sizeof(T) <= 128 ? TN : 1;
+  constexpr int LINE = AT * 32 * (int)sizeof(T), UNITS = LINE / 16;    // a row's run of columns: bytes, 16-byte units
+  constexpr int ROWS = AT == 1 ? 32 : 16;
+  constexpr int WAVE_LDS = AT == 1 ? std::max(ROWS * LINE, 256) : ROWS * LINE + AT * 32 * 8;
+  static_assert(TN <= 2 && WAVE_LDS <= 4096, "a lane holds one column's scale; the stages leave each wave 4 KB");
   // (arrays of their own: the compiler then knows which stage a DMA writes, and a read of another one waits for none)
   __shared__ __align__(128) signed char x0[BM * 64], x1[BM * 64], x2[BM * 64], x3[BM * 64], w0[BN * 64], w1[BN * 64], w2[BN * 64], w3[BN * 64];
   __shared__ __align__(128) signed char turned[WM * WN * WAVE_LDS];
@@ -218,9 +221,11 @@ __global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m
     acc[i % TN][i / TN] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[s][i % TN], fx[s][i / TN], acc[i % TN][i / TN], 0, 0, 0);
   };
   // A lane holds one row of y for each b, and of each 32 columns the quads 8 q + 4 c .. + 3.  Stored from there an instruction would write 32 bytes of
-  // each of 32 rows: each wave turns its rows over in LDS, ROWS at a time, and stores whole runs of columns (62500 x 600 float32: 89 us without, 73 us
-  // so).  PAST: the tiles of large products are stored past the caches, whose write-back of 33 MB or more otherwise meets the next tiles' reads (62500 x
-  // 600 float32 75 -> 67 us; 4096 x 4096 bfloat16, K = 512 20.9 -> 18.4 us; 8192 x 8192, K = 4096 293 -> 276 us).
+  // each of 32 rows: each wave turns its rows over in LDS and stores runs of 128 bytes (62500 x 600 float32, K = 602: 89 us without).  32 rows at a
+  // time where a tile's row is 128 bytes: with longer runs of fewer rows only some lanes write, and the LDS is what the epilogue waits for (68 us so,
+  // 58 us with all lanes writing).
+  // PAST: the tiles of large products are stored past the caches, whose write-back of 33 MB or more otherwise meets the next tiles' reads (4096 x 4096
+  // bfloat16, K = 512 20.9 -> 18.4 us; 8192 x 8192, K = 4096 293 -> 276 us).
   // Scales and bias are loaded before the first store: a load behind it would wait for it (one counter for both, in order).
   signed char* turn = turned + wave * WAVE_LDS;
   auto finish = [&](int t) {
@@ -230,7 +235,6 @@ __global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m
     place(t, m0, n0);
     m0 += wm * TM * 32;
     n0 += wn * TN * 32;
-    float* cols = (float*)(turn + ROWS * LINE);                        // [TN 32] scales, [TN 32] biases
     float sx[TM], sw = 0.f, bias = 0.f;
     if (lane < TN * 32) {
       const int n = min(n0 + lane, A.N - 1);
@@ -243,57 +247,73 @@ __global__ void __launch_bounds__(WM * WN * 64) k_i8_tile(i8_args A, int tiles_m
       const int64_t row = i8_row(A, min(m0 + b * 32 + r, A.M - 1), ok);
       sx[b] = ok ? A.sx[row] : 0.f;
     }
-    if (lane < TN * 32) {
-      cols[lane] = sw;
-      cols[TN * 32 + lane] = bias;
-    }
-    __builtin_amdgcn_wave_barrier();
     const bool full = m0 + TM * 32 <= A.M && n0 + TN * 32 <= A.N;
 #pragma unroll
-    for (int b = 0; b < TM; ++b) {
-      float v[TN * 4][4];
+    for (int a = 0; a < TN; a += AT) {
+      // scales [AT 32] and biases [AT 32]: behind the rows, or (one tile at a time) in their place, from where each lane takes its own first
+      float* cols = (float*)(turn + (AT == 1 ? 0 : ROWS * LINE));
+      const int mine = lane - a * 32;
+      __builtin_amdgcn_wave_barrier();
+      if (mine >= 0 && mine < AT * 32) {
+        cols[mine] = sw;
+        cols[AT * 32 + mine] = bias;
+      }
+      __builtin_amdgcn_wave_barrier();
+      float w[AT == 1 ? 4 : 1][4], d[AT == 1 ? 4 : 1][4];
+      if constexpr (AT == 1) {
 #pragma unroll
-      for (int u = 0; u < TN * 4; ++u) {
-        const int at = u * 8 + c * 4;
-        float w[4], d[4];
-        *(float4*)w = *(const float4*)(cols + at);
-        *(float4*)d = *(const float4*)(cols + TN * 32 + at);
-        const v16i32& s = acc[u >> 2][b];
-        const int q = (u & 3) * 4;
-        i8_values(A, v4i32{s[q], s[q + 1], s[q + 2], s[q + 3]}, sx[b], w, d, v[u]);
+        for (int u = 0; u < 4; ++u) {
+          *(float4*)w[u] = *(const float4*)(cols + u * 8 + c * 4);
+          *(float4*)d[u] = *(const float4*)(cols + 32 + u * 8 + c * 4);
+        }
+        __builtin_amdgcn_wave_barrier();
       }
 #pragma unroll
-      for (int h = 0; h < 32 / ROWS; ++h) {
-        const int rr = r & (ROWS - 1);
-        if (ROWS == 32 || r / ROWS == h) {
+      for (int b = 0; b < TM; ++b) {
+        float v[AT * 4][4];
 #pragma unroll
-          for (int u = 0; u < TN * 4; ++u) {
-            const int at = (u * 8 + c * 4) * (int)sizeof(T);
-            row_store<T, 4>((T*)(turn + rr * LINE + ((at >> 4) ^ (rr & (UNITS - 1))) * 16 + (at & 15)), v[u]);
+        for (int u = 0; u < AT * 4; ++u) {
+          if constexpr (AT > 1) {
+            *(float4*)w[0] = *(const float4*)(cols + u * 8 + c * 4);
+            *(float4*)d[0] = *(const float4*)(cols + AT * 32 + u * 8 + c * 4);
           }
+          const v16i32& s = acc[a + (u >> 2)][b];
+          const int q = (u & 3) * 4;
+          i8_values(A, v4i32{s[q], s[q + 1], s[q + 2], s[q + 3]}, sx[b], w[AT == 1 ? u : 0], d[AT == 1 ? u : 0], v[u]);
         }
-        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int it = 0; it < ROWS * UNITS / 64; ++it) {
-          const int line = it * (64 / UNITS) + lane / UNITS, unit = lane % UNITS;
-          const int64_t m = m0 + b * 32 + h * ROWS + line;
-          const int n = n0 + unit * E;
-          const T* from = (const T*)(turn + line * LINE + (unit ^ (line & (UNITS - 1))) * 16);
-          T* yp = (T*)A.y + m * A.ldy + n;
-          if (full) {
-            if constexpr (PAST) __builtin_nontemporal_store(*(const i8_piece*)from, (i8_piece*)yp);
-            else __builtin_memcpy(yp, from, 16);
-          } else if (m < A.M && n < A.N) {
-            if (n + E <= A.N) {
-              __builtin_memcpy(yp, from, 16);
-            } else {
-              for (int i = 0; i < E; ++i)
-                if (n + i < A.N) yp[i] = from[i];
+        for (int h = 0; h < 32 / ROWS; ++h) {
+          const int rr = r & (ROWS - 1);
+          if (ROWS == 32 || r / ROWS == h) {
+#pragma unroll
+            for (int u = 0; u < AT * 4; ++u) {
+              const int at = (u * 8 + c * 4) * (int)sizeof(T);
+              row_store<T, 4>((T*)(turn + rr * LINE + ((at >> 4) ^ (rr & (UNITS - 1))) * 16 + (at & 15)), v[u]);
             }
           }
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int it = 0; it < ROWS * UNITS / 64; ++it) {
+            const int line = it * (64 / UNITS) + lane / UNITS, unit = lane % UNITS;
+            const int64_t m = m0 + b * 32 + h * ROWS + line;
+            const int n = n0 + a * 32 + unit * E;
+            const T* from = (const T*)(turn + line * LINE + (unit ^ (line & (UNITS - 1))) * 16);
+            T* yp = (T*)A.y + m * A.ldy + n;
+            if (full) {
+              if constexpr (PAST) __builtin_nontemporal_store(*(const i8_piece*)from, (i8_piece*)yp);
+              else __builtin_memcpy(yp, from, 16);
+            } else if (m < A.M && n < A.N) {
+              if (n + E <= A.N) {
+                __builtin_memcpy(yp, from, 16);
+              } else {
+                for (int i = 0; i < E; ++i)
+                  if (n + i < A.N) yp[i] = from[i];
+              }
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
