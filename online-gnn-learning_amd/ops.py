@@ -3291,13 +3291,18 @@ def _row_device(what, first, *others):
     return dev
 
 
-def _row_launch(dev, name, fn, *args, meta=None):
+def _row_launch(dev, name, fn, *args, **meta):
     """``_launch`` on ``dev``'s current stream, whichever device is current."""
-    if dev.index == torch._C._cuda_getDevice():
-        _launch(name, fn, *args, _stream(), meta=meta)
-    else:
+    index = dev.index
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             _launch(name, fn, *args, _stream(), meta=meta)
+    elif _PROFILE is not None or _DEFERRED:
+        _launch(name, fn, *args, _stream(), meta=meta)
+    else:                                                  # (a small call is bound by the host: nothing in between)
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if st:
+            check(st, name)
 
 
 def _row_mat(what, x):
@@ -3321,7 +3326,7 @@ def _row_empty(rows, cols, dtype, device):
     """[rows, cols] view of an allocation with ``padded_ld`` columns (``empty_mat`` for any row type)."""
     ld = padded_ld(cols)
     t = torch.empty((rows, ld), dtype=dtype, device=device)
-    return t if ld == cols else t[:, :cols]
+    return t if ld == cols else t.as_strided((rows, cols), (ld, 1))
 
 
 class QuantRows:
@@ -3401,9 +3406,9 @@ def quant_rows_write(cache, x, slots=None, start=0):
     h = _lib.lib()
     nb = 0 if slots is None else h.ogl_quant_rows_workspace_bytes(m, n, 1)
     ws = torch.empty(nb // 4, dtype=torch.int32, device=dev) if nb else None
-    _row_launch(dev, "ogl_quant_rows_write", h.ogl_quant_rows_write, _ptr(x), _ld(x), _ROW_TYPES[x.dtype], m, cache.width, _ptr(slots), start,
-                _ptr(cache.codes), cache.ld, cache.format, _ptr(cache.scales), n, cache.group, _ptr(ws), nb,
-                meta=dict(m=m, width=cache.width))
+    _row_launch(dev, "ogl_quant_rows_write", h.ogl_quant_rows_write, x.data_ptr(), _ld(x), _ROW_TYPES[x.dtype], m, cache.width, _ptr(slots), start,
+                cache.codes.data_ptr(), cache.ld, cache.format, cache.scales.data_ptr(), n, cache.group, _ptr(ws), nb,
+                m=m, width=cache.width)
     return cache
 
 
@@ -3416,9 +3421,9 @@ def quant_rows_read(cache, rows=None, dtype=torch.float32):
     m = cache.n if rows is None else _row_ids(what, rows, dev).numel()
     out = _row_empty(m, cache.width, dtype, dev)
     if m:
-        _row_launch(dev, "ogl_quant_rows_read", _lib.lib().ogl_quant_rows_read, _ptr(cache.codes), cache.ld, cache.format,
-                    _ptr(cache.scales), cache.n, cache.width, cache.group, _ptr(rows), m, _ptr(out), out.stride(0), _ROW_TYPES[dtype],
-                    meta=dict(m=m, width=cache.width))
+        _row_launch(dev, "ogl_quant_rows_read", _lib.lib().ogl_quant_rows_read, cache.codes.data_ptr(), cache.ld, cache.format,
+                    cache.scales.data_ptr(), cache.n, cache.width, cache.group, _ptr(rows), m, out.data_ptr(), out.stride(0), _ROW_TYPES[dtype],
+                    m=m, width=cache.width)
     return out
 
 
@@ -3475,9 +3480,9 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32, o
     if x.n == 0:
         raise ValueError("%s: rows of an empty table" % what)
     b = bias.contiguous() if bias is not None else None
-    _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, _ptr(x.codes), x.ld, _ptr(x.scales), _ptr(x_rows), x.n, M, K,
-                _ptr(w.codes), w.ld, _ptr(w.scales), N, _ptr(b), int(bool(relu)), _ptr(y), _ld(y), _ROW_TYPES[dtype],
-                meta=dict(M=M, N=N, K=K))
+    _row_launch(dev, "ogl_linear_i8", _lib.lib().ogl_linear_i8, x.codes.data_ptr(), x.ld, x.scales.data_ptr(), _ptr(x_rows), x.n, M, K,
+                w.codes.data_ptr(), w.ld, w.scales.data_ptr(), N, _ptr(b), int(bool(relu)), y.data_ptr(), _ld(y), _ROW_TYPES[dtype],
+                M=M, N=N, K=K)
     return y
 
 
@@ -3529,7 +3534,7 @@ def group_norm_fwd(x, num_groups, weight, bias, eps, act, want_stats):
         mean = stats.data_ptr() if want_stats else None
         _row_launch(x.device, "ogl_group_norm_fwd", _lib.lib().ogl_group_norm_fwd, x.data_ptr(), xb, xl, t, B, L, C, G, _ptr(weight), _ptr(bias),
                     0 if p is None else _ROW_TYPES[p.dtype], eps, act, y.data_ptr(), yb, yl, mean, mean + 4 * B * G if want_stats else None, _ptr(ws),
-                    max(nb, 0), meta=dict(B=B, L=L, C=C, G=G))
+                    max(nb, 0), B=B, L=L, C=C, G=G)
     return y, stats
 
 
@@ -3552,7 +3557,7 @@ def group_norm_bwd(dy, x, num_groups, weight, bias, stats, act, want_dx=True, wa
     mean = stats.data_ptr()
     _row_launch(x.device, "ogl_group_norm_bwd", _lib.lib().ogl_group_norm_bwd, dy.data_ptr(), gb, gl, x.data_ptr(), xb, xl, t, B, L, C, G, _ptr(weight),
                 _ptr(bias), 0 if p is None else _ROW_TYPES[p.dtype], act, mean, mean + 4 * B * G, _ptr(dx), yb, yl, _ptr(dw), _ptr(db), ws.data_ptr(), nb,
-                meta=dict(B=B, L=L, C=C, G=G))
+                B=B, L=L, C=C, G=G)
     return dx, dw, db
 
 
