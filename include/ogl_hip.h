@@ -814,7 +814,7 @@ enum { OGL_ROWS_INT8 = 0, OGL_ROWS_E4M3 = 1 };
  * A group that holds an infinity or a NaN: s = NaN, codes 0 — it reads back as NaN.
  *   write  row i of x goes to slots[i], or to start + i where slots is NULL (then [start, start + m) has to lie inside the cache).  Slots outside
  *          [0, n) are skipped; of rows with the same slot the LAST stands.  The workspace needs no particular contents and keeps none.
- *          m * groups and m below 2^31.
+ *          m * groups and m below 2^31, n below 2^32, rows of x and of codes less than 2^31 elements apart.
  *   read   out[i, :] = fl32(code * s), rounded once to out_type, of row rows[i] (NULL: row i, m <= n); ids outside [0, n) yield zero rows.
  * Writes and reads of the same rows are ordered by their stream only. */
 int64_t ogl_quant_rows_workspace_bytes(int64_t m, int64_t n, int by_slots);
@@ -827,7 +827,7 @@ int ogl_quant_rows_read(const void* codes, int64_t ldc, int format, const float*
 /* y[m, n] = act((sx[r] sw[n]) * sum_k x[r, k] w[n, k] + bias[n]), r = rows[m] (NULL: m, then M <= nrows): the product of two caches in int8 with
  * one scale a row (a weight's rows are its output channels), act = relu or none, y in y_type.  The sum is exact; everything behind it is float32.
  * x [nrows, ldx], w [N, ldw]: 64-byte aligned, ld a multiple of 64, zeros behind column K in at least one of them; 1 <= K < 131072.
- * Rows outside [0, nrows) count as zero rows (y = act(bias)). */
+ * Rows outside [0, nrows) count as zero rows (y = act(bias)).  Tables of 2^38 bytes and more: OGL_EINVAL. */
 int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const int64_t* rows, int64_t nrows, int64_t M, int K, const void* w, int64_t ldw,
                   const float* sw, int N, const float* bias, int relu, void* y, int64_t ldy, int y_type, ogl_stream_t stream);
 

@@ -374,7 +374,7 @@ __device__ __forceinline__ void gn_lds_put(float* p, const float (&v)[V]) {
   for (int e = 0; e < V; e += 4) *(float4*)(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
 }
 
-// lanes of a wave that work on one of `groups` groups together
+// lanes of a wave that work on one of `groups` groups (or channels) together
 __device__ __forceinline__ int gn_group_lanes(int groups) {
   int t = 64;
   while (t > 1 && t * groups > GN_THREADS) t >>= 1;
@@ -441,18 +441,26 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
       }
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {               // (entry c of position 0 is this thread's from here on)
-      const float first = S.a[c];
-      float s = 0.f, q = S.q[c];
-      const int most = min(A.rp, rows), whole = rows / A.rp, rest = rows - whole * A.rp;
-      for (int ri = 1; ri < most; ++ri) {
-        const float n = (float)(whole + (ri < rest)), d = S.a[ri * A.nvec * V + c] - first;
-        s = __builtin_fmaf(n, d, s);
-        q += __builtin_fmaf(n * d, d, S.q[ri * A.nvec * V + c]);
-      }
+    const int lanes = gn_group_lanes(P.W), lane = threadIdx.x & (lanes - 1);
+    const int most = min(A.rp, rows), whole = rows / A.rp, rest = rows - whole * A.rp;
+    for (int c0 = 0; c0 < P.W; c0 += GN_THREADS / lanes) {
+      const int c = c0 + threadIdx.x / lanes;                          // (its entry of position 0 is this team's from here on)
+      const bool live = c < P.W;
+      const float first = live ? S.a[c] : 0.f;
+      float s = 0.f, q = 0.f;
+      if (live)
+        for (int ri = lane; ri < most; ri += lanes) {
+          const float n = (float)(whole + (ri < rest)), d = S.a[ri * A.nvec * V + c] - first;
+          s = __builtin_fmaf(n, d, s);
+          q += __builtin_fmaf(n * d, d, S.q[ri * A.nvec * V + c]);
+        }
+      s = row_team_sum(s, lanes);
+      q = row_team_sum(q, lanes);
       const float d = s * in;
-      S.a[c] = first + d;
-      S.q[c] = gn_not_negative(__builtin_fmaf(-d, s, q));
+      if (live && lane == 0) {
+        S.a[c] = first + d;
+        S.q[c] = gn_not_negative(__builtin_fmaf(-d, s, q));
+      }
     }
   } else {
     float k = 0.f, s = 0.f, q = 0.f;
@@ -555,25 +563,28 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
   }
 }
 
-// a block a sample window
+// a block a sample window, block x of grid_b taking every grid_b-th sample
 template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
   __shared__ gn_stats_lds S;
   __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
-  const int64_t b = A.by_nw.div(blockIdx.x);
-  const gn_place P = gn_where(A, b, (int)(blockIdx.x - (uint32_t)b * A.nw), 0);
+  const int64_t x = A.by_nw.div(blockIdx.x);
+  gn_place P = gn_where(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
-  gn_apply_rows<T, V, WIDE, PIECE>(A, P, 0, A.L, mean, rstd, [&]() {
-    gn_block_stats<T, V, WIDE, PIECE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
-      const float r = 1.f / sqrtf(m2 * inv + A.eps);
-      mean[g] = mu;
-      rstd[g] = r;
-      if (A.mean) {
-        A.mean[b * A.G + P.g0 + g] = mu;
-        A.rstd[b * A.G + P.g0 + g] = r;
-      }
+  for (int64_t b = x; b < A.B; b += A.grid_b) {                        // (the statistics' barriers keep the rounds apart)
+    P.b = b;
+    gn_apply_rows<T, V, WIDE, PIECE>(A, P, 0, A.L, mean, rstd, [&]() {
+      gn_block_stats<T, V, WIDE, PIECE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
+        const float r = 1.f / sqrtf(m2 * inv + A.eps);
+        mean[g] = mu;
+        rstd[g] = r;
+        if (A.mean) {
+          A.mean[b * A.G + P.g0 + g] = mu;
+          A.rstd[b * A.G + P.g0 + g] = r;
+        }
+      });
     });
-  });
+  }
 }
 
 // tiles of positions: part[(b, group), tile] = (mean, M2)
@@ -723,6 +734,27 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
   while (r < r1) rows(std::integral_constant<int, 1>());
 }
 
+// the window's channel sums over the block's positions -> out[0: dz, 1: dz h][C]; every thread takes part
+template <int V>
+__device__ __forceinline__ void gn_fold_window(const gn_args& A, const gn_place& P, const float* cz, const float* ch, float* out) {
+  const int lanes = gn_group_lanes(P.W), lane = threadIdx.x & (lanes - 1);
+  for (int c0 = 0; c0 < P.W; c0 += GN_THREADS / lanes) {
+    const int c = c0 + threadIdx.x / lanes;
+    float a = 0.f, d = 0.f;
+    if (c < P.W)
+      for (int q = lane; q < A.rp; q += lanes) {
+        a += cz[q * A.nvec * V + c];
+        d += ch[q * A.nvec * V + c];
+      }
+    a = row_team_sum(a, lanes);
+    d = row_team_sum(d, lanes);
+    if (c < P.W && lane == 0) {
+      out[c] = a;
+      out[A.C + c] = d;
+    }
+  }
+}
+
 // a block a sample window, block x of grid_b taking every grid_b-th sample: part[x][0: dz, 1: dz h][C] holds the sums over its samples
 template <typename T, int V, bool WIDE, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
@@ -788,12 +820,12 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
         const bool live = g < P.groups;
         float s1 = 0.f, s2 = 0.f;
         if (live) {
-          for (int ri = 0; ri < (WIDE ? 1 : A.rp); ++ri)
-            for (int c = lane; c < (WIDE ? GN_THREADS : A.Cg); c += lanes) {
-              const int at = WIDE ? c : ri * A.nvec * V + g * A.Cg + c;
-              s1 += cz[at];
-              s2 += ch[at];
-            }
+          for (int i = lane; i < (WIDE ? GN_THREADS : A.rp * A.Cg); i += lanes) {
+            const int ri = WIDE ? 0 : (int)A.by_cg.div((uint32_t)i);
+            const int at = WIDE ? i : ri * A.nvec * V + g * A.Cg + i - ri * A.Cg;
+            s1 += cz[at];
+            s2 += ch[at];
+          }
         }
         s1 = row_team_sum(s1, lanes);
         s2 = row_team_sum(s2, lanes);
@@ -827,15 +859,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
     gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, th);
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {
-    float a = 0.f, d = 0.f;
-    for (int q = 0; q < A.rp; ++q) {
-      a += cz[q * A.nvec * V + c];
-      d += ch[q * A.nvec * V + c];
-    }
-    out[c] = a;
-    out[A.C + c] = d;
-  }
+  gn_fold_window<V>(A, P, cz, ch, out);
 }
 
 // tiles of positions: part[b, tile][0: dz, 1: dz h][C]
@@ -875,15 +899,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
       gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, sh);
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < P.W; c += GN_THREADS) {
-      float a = 0.f, d = 0.f;
-      for (int q = 0; q < A.rp; ++q) {
-        a += cz[q * A.nvec * V + c];
-        d += ch[q * A.nvec * V + c];
-      }
-      out[c] = a;
-      out[A.C + c] = d;
-    }
+    gn_fold_window<V>(A, P, cz, ch, out);
   }
 }
 
@@ -1032,7 +1048,8 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
   A.by_nvec = ogl_div::make((uint32_t)A.nvec);
   A.by_nw = ogl_div::make((uint32_t)A.nw);
   A.by_tiles = ogl_div::make((uint32_t)A.tiles);
-  A.grid_b = (int)std::min<int64_t>(A.B, std::max<int64_t>(1, 2048 / A.nw));
+  // samples side by side: the backward's blocks each leave 2 C partial sums, the forward's only have to stay below 2^32 threads
+  A.grid_b = (int)std::min<int64_t>(A.B, std::max<int64_t>(1, (backward ? 2048 : 1 << 23) / A.nw));
   if (backward) {
     P.part = (A.tiles == 1 ? (int64_t)A.grid_b : A.B * A.tiles) * 2 * A.C;
     P.sums = A.tiles == 1 ? 0 : A.B * A.G * 2;
@@ -1084,9 +1101,9 @@ static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
     return OGL_OK;
   }
   if (A.tiles == 1) {
-    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true, cut>), A.B * A.nw);
-    else if (P.even) GN_LAUNCH((k_gn_sample_fwd<T, V, false, whole>), A.B * A.nw);
-    else GN_LAUNCH((k_gn_sample_fwd<T, V, false, cut>), A.B * A.nw);
+    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true, cut>), (int64_t)A.grid_b * A.nw);
+    else if (P.even) GN_LAUNCH((k_gn_sample_fwd<T, V, false, whole>), (int64_t)A.grid_b * A.nw);
+    else GN_LAUNCH((k_gn_sample_fwd<T, V, false, cut>), (int64_t)A.grid_b * A.nw);
     return OGL_OK;
   }
   const int64_t grid = A.B * A.nw * A.tiles;

@@ -415,6 +415,8 @@ extern "C" int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const 
   if (M < 0 || N < 0 || K < 1 || K > 131071 || nrows < 0 || ldx < K || ldw < K || ldx % 64 || ldw % 64 || ldy < N || y_type < OGL_F32 || y_type > OGL_F16)
     return OGL_EINVAL;
   if (!rows && M > nrows) return OGL_EINVAL;
+  const double most = 4294967296.;                                    // offsets count 64 bytes in 32 bits
+  if ((double)nrows * (double)(ldx / 64) >= most || (double)N * (double)(ldw / 64) >= most) return OGL_EINVAL;
   if (M == 0 || N == 0) return OGL_OK;
   if (!w || !sw || !y || ((uintptr_t)w & 63) || ((uintptr_t)y & (y_type == OGL_F32 ? 3 : 1)) || nrows == 0 || !x || !sx || ((uintptr_t)x & 63))
     return OGL_EINVAL;
