@@ -349,6 +349,7 @@ struct gn_place {
   int win, tile, g0, groups, c0, W, j, ri;
   bool on;
 };
+template <int NT>
 __device__ __forceinline__ gn_place gn_where(const gn_args& A, int64_t b, int win, int tile) {
   gn_place P;
   P.b = b;
@@ -364,9 +365,10 @@ __device__ __forceinline__ gn_place gn_where(const gn_args& A, int64_t b, int wi
   return P;
 }
 
+template <int NT>
 struct __align__(16) gn_stats_lds {
-  float a[GN_THREADS * 8], q[GN_THREADS * 8];                          // [rp][nvec V] sums around a pivot, then (mean, M2) of a channel; WIDE: of a thread
-  int count[GN_THREADS];                                               // WIDE: values of the thread
+  float a[NT * 8], q[NT * 8];                          // [rp][nvec V] sums around a pivot, then (mean, M2) of a channel; WIDE: of a thread
+  int count[NT];                                               // WIDE: values of the thread
 };
 template <int V>
 __device__ __forceinline__ void gn_lds_put(float* p, const float (&v)[V]) {
@@ -375,17 +377,18 @@ __device__ __forceinline__ void gn_lds_put(float* p, const float (&v)[V]) {
 }
 
 // lanes of a wave that work on one of `groups` groups (or channels) together
+template <int NT>
 __device__ __forceinline__ int gn_group_lanes(int groups) {
   int t = 64;
-  while (t > 1 && t * groups > GN_THREADS) t >>= 1;
+  while (t > 1 && t * groups > NT) t >>= 1;
   return t;
 }
 
 // (mean, M2) of each of the block's groups over positions r0 .. r1, handed to `done(group of the window, mean, M2)` by one lane a group.
 // NARROW: a thread's sums and squares around its first value, from them its (mean, M2); those of a channel's threads joined around the first one's mean,
 // then those of a group's channels likewise.
-template <typename T, int V, bool WIDE, typename PIECE, typename F>
-__device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place& P, int r0, int r1, gn_stats_lds& S, F done) {
+template <typename T, int V, bool WIDE, typename PIECE, int NT, typename F>
+__device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place& P, int r0, int r1, gn_stats_lds<NT>& S, F done) {
   const T* xp = (const T*)A.x + P.b * A.xb + P.c0 + (int64_t)r0 * A.xl;
   const int rows = r1 - r0;
   const float in = 1.f / (float)rows;
@@ -441,9 +444,9 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
       }
     }
     __syncthreads();
-    const int lanes = gn_group_lanes(P.W), lane = threadIdx.x & (lanes - 1);
+    const int lanes = gn_group_lanes<NT>(P.W), lane = threadIdx.x & (lanes - 1);
     const int most = min(A.rp, rows), whole = rows / A.rp, rest = rows - whole * A.rp;
-    for (int c0 = 0; c0 < P.W; c0 += GN_THREADS / lanes) {
+    for (int c0 = 0; c0 < P.W; c0 += NT / lanes) {
       const int c = c0 + threadIdx.x / lanes;                          // (its entry of position 0 is this team's from here on)
       const bool live = c < P.W;
       const float first = live ? S.a[c] : 0.f;
@@ -465,7 +468,7 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
   } else {
     float k = 0.f, s = 0.f, q = 0.f;
     int n = 0;
-    for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
+    for (int j = threadIdx.x; j < A.nvec; j += NT) {
       const int have = P.W - j * V;
       for (int r = 0; r < rows; ++r) {
         float v[V];
@@ -487,8 +490,8 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
     S.count[threadIdx.x] = n;
   }
   __syncthreads();
-  const int lanes = WIDE ? 64 : gn_group_lanes(P.groups);
-  const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
+  const int lanes = WIDE ? 64 : gn_group_lanes<NT>(P.groups);
+  const int lane = threadIdx.x & (lanes - 1), per = NT / lanes;
   for (int q0 = 0; q0 < P.groups; q0 += per) {
     const int g = q0 + threadIdx.x / lanes;
     const bool live = g < P.groups;
@@ -496,7 +499,7 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
     const float total = (float)A.Cg * (float)rows, first = live ? S.a[at] : 0.f;
     float a = 0.f, m2 = 0.f;
     if (live)
-      for (int c = lane; c < (WIDE ? GN_THREADS : A.Cg); c += lanes) {
+      for (int c = lane; c < (WIDE ? NT : A.Cg); c += lanes) {
         const float n = WIDE ? (float)S.count[c] : (float)rows, d = S.a[at + c] - first;
         if (n > 0.f) {
           a = __builtin_fmaf(n, d, a);
@@ -513,7 +516,7 @@ __device__ __forceinline__ void gn_block_stats(const gn_args& A, const gn_place&
 }
 
 // y of positions r0 .. r1 from the window's statistics, which `stats` (called once by every thread) puts into LDS while the first loads are on their way
-template <typename T, int V, bool WIDE, typename PIECE, typename F>
+template <typename T, int V, bool WIDE, typename PIECE, int NT, typename F>
 __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& P, int r0, int r1, const float* mean, const float* rstd, F stats) {
   constexpr int U = 2;
   typedef typename PIECE::raw raw_t;
@@ -528,7 +531,7 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
       if (have > 0 && first + u * step < r1) ahead[u] = C.fetch(xp + (int64_t)(first + u * step) * A.xl);
   }
   stats();
-  for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
+  for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? NT : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
     const PIECE C(have, P.W < V);
@@ -564,17 +567,17 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
 }
 
 // a block a sample window, block x of grid_b taking every grid_b-th sample
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
-  __shared__ gn_stats_lds S;
-  __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_sample_fwd(gn_args A) {
+  __shared__ gn_stats_lds<NT> S;
+  __shared__ float mean[NT], rstd[NT];
   const int64_t x = A.by_nw.div(blockIdx.x);
-  gn_place P = gn_where(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
+  gn_place P = gn_where<NT>(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
   for (int64_t b = x; b < A.B; b += A.grid_b) {                        // (the statistics' barriers keep the rounds apart)
     P.b = b;
-    gn_apply_rows<T, V, WIDE, PIECE>(A, P, 0, A.L, mean, rstd, [&]() {
-      gn_block_stats<T, V, WIDE, PIECE>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
+    gn_apply_rows<T, V, WIDE, PIECE, NT>(A, P, 0, A.L, mean, rstd, [&]() {
+      gn_block_stats<T, V, WIDE, PIECE, NT>(A, P, 0, A.L, S, [&](int g, float mu, float m2) {
         const float r = 1.f / sqrtf(m2 * inv + A.eps);
         mean[g] = mu;
         rstd[g] = r;
@@ -588,30 +591,30 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_fwd(gn_args A) {
 }
 
 // tiles of positions: part[(b, group), tile] = (mean, M2)
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_stats(gn_args A) {
-  __shared__ gn_stats_lds S;
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_stats(gn_args A) {
+  __shared__ gn_stats_lds<NT> S;
   const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
   const int64_t b = A.by_nw.div(u);
-  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
+  const gn_place P = gn_where<NT>(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
-  gn_block_stats<T, V, WIDE, PIECE>(A, P, r0, r1, S, [&](int g, float mu, float m2) {
+  gn_block_stats<T, V, WIDE, PIECE, NT>(A, P, r0, r1, S, [&](int g, float mu, float m2) {
     float2* o = (float2*)A.part + (b * A.G + P.g0 + g) * A.tiles + tile;
     *o = make_float2(mu, m2);
   });
 }
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_apply(gn_args A) {
-  __shared__ float mean[GN_THREADS], rstd[GN_THREADS];
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_apply(gn_args A) {
+  __shared__ float mean[NT], rstd[NT];
   const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
   const int64_t b = A.by_nw.div(u);
-  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
+  const gn_place P = gn_where<NT>(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows;
-  gn_apply_rows<T, V, WIDE, PIECE>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd, [&]() {
-    const int lanes = gn_group_lanes(P.groups);
-    const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
+  gn_apply_rows<T, V, WIDE, PIECE, NT>(A, P, r0, min(A.L, r0 + A.tile_rows), mean, rstd, [&]() {
+    const int lanes = gn_group_lanes<NT>(P.groups);
+    const int lane = threadIdx.x & (lanes - 1), per = NT / lanes;
     const float total = (float)A.Cg * (float)A.L;
     for (int q0 = 0; q0 < P.groups; q0 += per) {
       const int g = q0 + threadIdx.x / lanes;
@@ -735,10 +738,10 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
 }
 
 // the window's channel sums over the block's positions -> out[0: dz, 1: dz h][C]; every thread takes part
-template <int V>
+template <int V, int NT>
 __device__ __forceinline__ void gn_fold_window(const gn_args& A, const gn_place& P, const float* cz, const float* ch, float* out) {
-  const int lanes = gn_group_lanes(P.W), lane = threadIdx.x & (lanes - 1);
-  for (int c0 = 0; c0 < P.W; c0 += GN_THREADS / lanes) {
+  const int lanes = gn_group_lanes<NT>(P.W), lane = threadIdx.x & (lanes - 1);
+  for (int c0 = 0; c0 < P.W; c0 += NT / lanes) {
     const int c = c0 + threadIdx.x / lanes;
     float a = 0.f, d = 0.f;
     if (c < P.W)
@@ -756,12 +759,12 @@ __device__ __forceinline__ void gn_fold_window(const gn_args& A, const gn_place&
 }
 
 // a block a sample window, block x of grid_b taking every grid_b-th sample: part[x][0: dz, 1: dz h][C] holds the sums over its samples
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
-  __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];   // [rp][nvec V]; WIDE: s1, s2 of a thread
-  __shared__ float g1[GN_THREADS], g2[GN_THREADS];
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_sample_bwd(gn_args A) {
+  __shared__ __align__(16) float cz[NT * V], ch[NT * V];   // [rp][nvec V]; WIDE: s1, s2 of a thread
+  __shared__ float g1[NT], g2[NT];
   const int64_t x = A.by_nw.div(blockIdx.x);
-  const gn_place P = gn_where(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
+  const gn_place P = gn_where<NT>(A, x, (int)(blockIdx.x - (uint32_t)x * A.nw), 0);
   const float inv = 1.f / ((float)A.Cg * (float)A.L);
   float* out = A.part ? A.part + x * 2 * A.C + P.c0 : nullptr;
   float tz[V], th[V];
@@ -791,7 +794,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       }
     } else {
       float s1 = 0.f, s2 = 0.f;
-      for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
+      for (int j = threadIdx.x; j < A.nvec; j += NT) {
         const int have = P.W - j * V;
         float sz[V], sh[V];
         const PIECE C(have, false);
@@ -813,14 +816,14 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
     }
     if (A.write_dx) {                                                   // (the same for the whole grid)
       __syncthreads();
-      const int lanes = WIDE ? 64 : gn_group_lanes(P.groups);
-      const int lane = threadIdx.x & (lanes - 1), per = GN_THREADS / lanes;
+      const int lanes = WIDE ? 64 : gn_group_lanes<NT>(P.groups);
+      const int lane = threadIdx.x & (lanes - 1), per = NT / lanes;
       for (int q0 = 0; q0 < P.groups; q0 += per) {
         const int g = q0 + threadIdx.x / lanes;
         const bool live = g < P.groups;
         float s1 = 0.f, s2 = 0.f;
         if (live) {
-          for (int i = lane; i < (WIDE ? GN_THREADS : A.rp * A.Cg); i += lanes) {
+          for (int i = lane; i < (WIDE ? NT : A.rp * A.Cg); i += lanes) {
             const int ri = WIDE ? 0 : (int)A.by_cg.div((uint32_t)i);
             const int at = WIDE ? i : ri * A.nvec * V + g * A.Cg + i - ri * A.Cg;
             s1 += cz[at];
@@ -836,7 +839,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
       }
       __syncthreads();
       float s1[V], s2[V];
-      for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
+      for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? NT : A.nvec) {
         const int have = WIDE || P.on ? P.W - j * V : 0;
         if (have <= 0) break;
         const PIECE C(have, P.W < V);
@@ -859,17 +862,17 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_sample_bwd(gn_args A) {
     gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, th);
   }
   __syncthreads();
-  gn_fold_window<V>(A, P, cz, ch, out);
+  gn_fold_window<V, NT>(A, P, cz, ch, out);
 }
 
 // tiles of positions: part[b, tile][0: dz, 1: dz h][C]
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
-  __shared__ __align__(16) float cz[GN_THREADS * V], ch[GN_THREADS * V];
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_bwd_sums(gn_args A) {
+  __shared__ __align__(16) float cz[NT * V], ch[NT * V];
   const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
   const int64_t b = A.by_nw.div(u);
-  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
+  const gn_place P = gn_where<NT>(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
   const T* xp = (const T*)A.x + b * A.xb + P.c0;
   const T* gp = (const T*)A.dy + b * A.gb + P.c0;
@@ -877,7 +880,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
   gn_cols<V> K;
   float sz[V], sh[V];
   if constexpr (WIDE) {
-    for (int j = threadIdx.x; j < A.nvec; j += GN_THREADS) {
+    for (int j = threadIdx.x; j < A.nvec; j += NT) {
       const int have = P.W - j * V;
       const PIECE C(have, false);
       gn_columns<T, V, PIECE>(A, b, P.c0 + j * V, C, K);
@@ -899,7 +902,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_sums(gn_args A) {
       gn_lds_put<V>(ch + (P.ri * A.nvec + P.j) * V, sh);
     }
     __syncthreads();
-    gn_fold_window<V>(A, P, cz, ch, out);
+    gn_fold_window<V, NT>(A, P, cz, ch, out);
   }
 }
 
@@ -958,17 +961,17 @@ __global__ void __launch_bounds__(1024) k_gn_fold(gn_args A, int64_t groups, int
   }
 }
 
-template <typename T, int V, bool WIDE, typename PIECE>
-__global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
+template <typename T, int V, bool WIDE, typename PIECE, int NT>
+__global__ void __launch_bounds__(NT) k_gn_bwd_apply(gn_args A) {
   const uint32_t u = A.by_tiles.div(blockIdx.x);
   const int tile = (int)(blockIdx.x - u * A.tiles);
   const int64_t b = A.by_nw.div(u);
-  const gn_place P = gn_where(A, b, (int)(u - (uint32_t)b * A.nw), tile);
+  const gn_place P = gn_where<NT>(A, b, (int)(u - (uint32_t)b * A.nw), tile);
   const int r0 = tile * A.tile_rows, r1 = min(A.L, r0 + A.tile_rows);
   const T* xp = (const T*)A.x + b * A.xb + P.c0;
   const T* gp = (const T*)A.dy + b * A.gb + P.c0;
   T* dp = (T*)A.y + b * A.yb + P.c0;
-  for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? GN_THREADS : A.nvec) {
+  for (int j = WIDE ? (int)threadIdx.x : P.j; j < A.nvec; j += WIDE ? NT : A.nvec) {
     const int have = WIDE || P.on ? P.W - j * V : 0;
     if (have <= 0) return;
     const PIECE C(have, P.W < V);
@@ -989,6 +992,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_bwd_apply(gn_args A) {
 struct gn_plan {
   bool rows, block, wide;
   bool even;                   // maps: every window is whole pieces
+  int threads;                 // maps: of a block
   int nv, r;                   // rows: pieces a lane, rows a team
   int64_t part, sums;          // floats of workspace
 };
@@ -1020,24 +1024,28 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
     A.by_g = ogl_div::make((uint32_t)A.G);
     return P;
   }
-  // Windows of whole groups, at most 256 pieces wide, that keep most threads busy (pieces x positions side by side of 256) and waste least at the
-  // last window; of equals the widest.  One group wider than that: WIDE.
+  // Small samples (up to 8 pieces a lane): a wave each, so that four times as many are on their way; a block's time goes into its steps' latencies, not
+  // into its loads.  62500 x 2 x 256 bfloat16 forward / backward 295 / 507 -> 105 / 151 us, 20000 x 8 x 96 float32 147 / 148 -> 49 / 73 us; samples of
+  // 2048 pieces are as fast in blocks (3000 x 16 x 512 float32 44 / 84 us, a wave each 50 / 86).
+  P.threads = (int64_t)A.L * ogl_cdiv(A.C, V) <= 512 && pieces <= 64 && A.B >= 1024 ? 64 : GN_THREADS;
+  // Windows of whole groups, at most a block's pieces wide, that keep most threads busy (pieces x positions side by side of a block) and waste least at
+  // the last window; of equals the widest.  One group wider than that: WIDE.
   P.wide = pieces > GN_THREADS;
   A.gw = 1;
   if (!P.wide) {
     double best = -1;
-    for (int gw = std::min(A.G, 256); gw >= 1; --gw) {
+    for (int gw = std::min(A.G, P.threads); gw >= 1; --gw) {
       const int nvec = (int)ogl_cdiv((int64_t)gw * A.Cg, V);
-      if (nvec > GN_THREADS) continue;
+      if (nvec > P.threads) continue;
       if (gw < A.G && (int64_t)gw * A.Cg * (16 / V) < 128) break;      // windows of less than a line
-      const double busy = (double)(GN_THREADS / nvec * nvec) / GN_THREADS * ((double)gw * A.Cg / ((double)nvec * V)) *
+      const double busy = (double)(P.threads / nvec * nvec) / P.threads * ((double)gw * A.Cg / ((double)nvec * V)) *
                           ((double)A.G / (double)(ogl_cdiv(A.G, gw) * gw));
       if (busy > best + 0.02) best = busy, A.gw = gw;
     }
   }
   A.nw = (int)ogl_cdiv(A.G, A.gw);
   A.nvec = (int)ogl_cdiv((int64_t)A.gw * A.Cg, V);
-  A.rp = P.wide ? 1 : GN_THREADS / A.nvec;
+  A.rp = P.wide ? 1 : P.threads / A.nvec;
   P.even = A.C % V == 0 && (int64_t)A.gw * A.Cg % V == 0;
   // a block a sample window where there are enough of them to fill the card or little to do in each; else tiles of 8 positions a thread or more
   const int64_t blocks = A.B * A.nw;
@@ -1049,7 +1057,7 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
   A.by_nw = ogl_div::make((uint32_t)A.nw);
   A.by_tiles = ogl_div::make((uint32_t)A.tiles);
   // samples side by side: the backward's blocks each leave 2 C partial sums, the forward's only have to stay below 2^32 threads
-  A.grid_b = (int)std::min<int64_t>(A.B, std::max<int64_t>(1, (backward ? 2048 : 1 << 23) / A.nw));
+  A.grid_b = (int)std::min<int64_t>(A.B, std::max<int64_t>(1, (!backward ? 1 << 23 : P.threads == 64 ? 4096 : 2048) / A.nw));
   if (backward) {
     P.part = (A.tiles == 1 ? (int64_t)A.grid_b : A.B * A.tiles) * 2 * A.C;
     P.sums = A.tiles == 1 ? 0 : A.B * A.G * 2;
@@ -1073,12 +1081,13 @@ extern "C" int64_t ogl_group_norm_workspace_bytes(int64_t B, int64_t L, int C, i
   return 4 * (P.part + P.sums);
 }
 
-#define GN_LAUNCH(K, GRID, ...)                                                                   \
-  do {                                                                                            \
-    const int64_t grid_ = (GRID);                                                                 \
-    if (grid_ * GN_THREADS > (int64_t)UINT32_MAX) return OGL_EINVAL;                               \
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(K), dim3((unsigned)grid_), dim3(GN_THREADS), 0, st, A);    \
+#define GN_LAUNCH_N(THREADS, K, GRID)                                                          \
+  do {                                                                                         \
+    const int64_t grid_ = (GRID);                                                              \
+    if (grid_ * (THREADS) > (int64_t)UINT32_MAX) return OGL_EINVAL;                            \
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(K), dim3((unsigned)grid_), dim3(THREADS), 0, st, A);    \
   } while (0)
+#define GN_LAUNCH(K, GRID) GN_LAUNCH_N(GN_THREADS, K, GRID)
 
 template <typename T, int V>
 static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
@@ -1101,20 +1110,23 @@ static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
     return OGL_OK;
   }
   if (A.tiles == 1) {
-    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true, cut>), (int64_t)A.grid_b * A.nw);
-    else if (P.even) GN_LAUNCH((k_gn_sample_fwd<T, V, false, whole>), (int64_t)A.grid_b * A.nw);
-    else GN_LAUNCH((k_gn_sample_fwd<T, V, false, cut>), (int64_t)A.grid_b * A.nw);
+    const int64_t grid = (int64_t)A.grid_b * A.nw;
+    if (P.wide) GN_LAUNCH((k_gn_sample_fwd<T, V, true, cut, GN_THREADS>), grid);
+    else if (P.threads == 64 && P.even) GN_LAUNCH_N(64, (k_gn_sample_fwd<T, V, false, whole, 64>), grid);
+    else if (P.threads == 64) GN_LAUNCH_N(64, (k_gn_sample_fwd<T, V, false, cut, 64>), grid);
+    else if (P.even) GN_LAUNCH((k_gn_sample_fwd<T, V, false, whole, GN_THREADS>), grid);
+    else GN_LAUNCH((k_gn_sample_fwd<T, V, false, cut, GN_THREADS>), grid);
     return OGL_OK;
   }
   const int64_t grid = A.B * A.nw * A.tiles;
   if (P.wide) {
-    GN_LAUNCH((k_gn_stats<T, V, true, cut>), grid);
-    GN_LAUNCH((k_gn_apply<T, V, true, cut>), grid);
+    GN_LAUNCH((k_gn_stats<T, V, true, cut, GN_THREADS>), grid);
+    GN_LAUNCH((k_gn_apply<T, V, true, cut, GN_THREADS>), grid);
   } else {
-    if (P.even) GN_LAUNCH((k_gn_stats<T, V, false, whole>), grid);
-    else GN_LAUNCH((k_gn_stats<T, V, false, cut>), grid);
-    if (P.even) GN_LAUNCH((k_gn_apply<T, V, false, whole>), grid);
-    else GN_LAUNCH((k_gn_apply<T, V, false, cut>), grid);
+    if (P.even) GN_LAUNCH((k_gn_stats<T, V, false, whole, GN_THREADS>), grid);
+    else GN_LAUNCH((k_gn_stats<T, V, false, cut, GN_THREADS>), grid);
+    if (P.even) GN_LAUNCH((k_gn_apply<T, V, false, whole, GN_THREADS>), grid);
+    else GN_LAUNCH((k_gn_apply<T, V, false, cut, GN_THREADS>), grid);
   }
   return OGL_OK;
 }
@@ -1142,14 +1154,17 @@ static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, h
 #undef GN_ROWS
     rows = A.chunks;
   } else if (A.tiles == 1) {
-    if (P.wide) GN_LAUNCH((k_gn_sample_bwd<T, V, true, cut>), (int64_t)A.grid_b * A.nw);
-    else if (P.even) GN_LAUNCH((k_gn_sample_bwd<T, V, false, whole>), (int64_t)A.grid_b * A.nw);
-    else GN_LAUNCH((k_gn_sample_bwd<T, V, false, cut>), (int64_t)A.grid_b * A.nw);
+    const int64_t grid = (int64_t)A.grid_b * A.nw;
+    if (P.wide) GN_LAUNCH((k_gn_sample_bwd<T, V, true, cut, GN_THREADS>), grid);
+    else if (P.threads == 64 && P.even) GN_LAUNCH_N(64, (k_gn_sample_bwd<T, V, false, whole, 64>), grid);
+    else if (P.threads == 64) GN_LAUNCH_N(64, (k_gn_sample_bwd<T, V, false, cut, 64>), grid);
+    else if (P.even) GN_LAUNCH((k_gn_sample_bwd<T, V, false, whole, GN_THREADS>), grid);
+    else GN_LAUNCH((k_gn_sample_bwd<T, V, false, cut, GN_THREADS>), grid);
     rows = A.grid_b;
   } else {
-    if (P.wide) GN_LAUNCH((k_gn_bwd_sums<T, V, true, cut>), A.B * A.nw * A.tiles);
-    else if (P.even) GN_LAUNCH((k_gn_bwd_sums<T, V, false, whole>), A.B * A.nw * A.tiles);
-    else GN_LAUNCH((k_gn_bwd_sums<T, V, false, cut>), A.B * A.nw * A.tiles);
+    if (P.wide) GN_LAUNCH((k_gn_bwd_sums<T, V, true, cut, GN_THREADS>), A.B * A.nw * A.tiles);
+    else if (P.even) GN_LAUNCH((k_gn_bwd_sums<T, V, false, whole, GN_THREADS>), A.B * A.nw * A.tiles);
+    else GN_LAUNCH((k_gn_bwd_sums<T, V, false, cut, GN_THREADS>), A.B * A.nw * A.tiles);
     rows = A.B * A.tiles;
     groups = A.write_dx ? A.B * A.G : 0;
   }
@@ -1158,9 +1173,9 @@ static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, h
   if (groups + folds > 0)
     hipLaunchKernelGGL(k_gn_fold<T>, dim3((unsigned)(groups + folds)), dim3(1024), 0, st, A, groups, rows, dw, db);
   if (groups > 0) {
-    if (P.wide) GN_LAUNCH((k_gn_bwd_apply<T, V, true, cut>), A.B * A.nw * A.tiles);
-    else if (P.even) GN_LAUNCH((k_gn_bwd_apply<T, V, false, whole>), A.B * A.nw * A.tiles);
-    else GN_LAUNCH((k_gn_bwd_apply<T, V, false, cut>), A.B * A.nw * A.tiles);
+    if (P.wide) GN_LAUNCH((k_gn_bwd_apply<T, V, true, cut, GN_THREADS>), A.B * A.nw * A.tiles);
+    else if (P.even) GN_LAUNCH((k_gn_bwd_apply<T, V, false, whole, GN_THREADS>), A.B * A.nw * A.tiles);
+    else GN_LAUNCH((k_gn_bwd_apply<T, V, false, cut, GN_THREADS>), A.B * A.nw * A.tiles);
   }
   return OGL_OK;
 }

@@ -110,6 +110,13 @@ def test_float32_every_shape(ops, shape, G):
     check(ops, shape, G, act="silu", seed=sum(shape))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,G", [((1030, 2, 8), 2), ((1030, 3, 9), 3), ((1024, 7, 40), 5), ((2050, 4, 6), 1), ((1500, 2, 250), 1), ((1100, 50, 12), 4),
+                                     ((1024, 2, 1000), 125), ((9001, 2, 5), 5)])
+def test_many_small_maps(ops, dtype, shape, G):
+    check(ops, shape, G, dtype, act="silu", seed=sum(shape))
+
+
 @pytest.mark.parametrize("act", [None, "relu", "gelu"])
 @pytest.mark.parametrize("shape,G", [((65, 96), 6), ((2, 40, 64), 8), ((1, 1500, 48), 4), ((3, 2, 4500), 1)])
 def test_activations(ops, act, shape, G):
