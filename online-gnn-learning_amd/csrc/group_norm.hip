@@ -52,12 +52,14 @@ struct gn_team {
 // over a team, the same bits in every lane; every lane of the wave takes part
 __device__ __forceinline__ float gn_span_sum(float v, const gn_args& A, const gn_team& t) {
   if ((A.lanes & (A.lanes - 1)) == 0) return row_team_sum(v, A.lanes);
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < A.lanes; o <<= 1) {
-    const float u = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane + o) * 4, __builtin_bit_cast(int, v)));
-    v += t.pos + o < A.lanes ? u : 0.f;
-  }
-  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute((lane - t.pos) * 4, __builtin_bit_cast(int, v)));
+  const int at = (threadIdx.x & 63) * 4;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1)
+    if (o < A.lanes) {
+      const float u = __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(at + o * 4, __builtin_bit_cast(int, v)));
+      v += t.pos + o < A.lanes ? u : 0.f;
+    }
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(at - t.pos * 4, __builtin_bit_cast(int, v)));
 }
 
 // The normal distribution function at z, and e^(-z^2 / 2): Phi(-|z|) = erfc(x) / 2 at x = |z| / sqrt 2 by the polynomial of Abramowitz and Stegun
@@ -73,25 +75,36 @@ __device__ __forceinline__ float gn_phi(float z, float& e) {
   const float q = 0.5f * t * p * e;
   return z < 0.f ? q : 1.f - q;
 }
-__device__ __forceinline__ float gn_act(float z, int act) {
+template <int ACT>
+__device__ __forceinline__ float gn_act(float z) {
   float e;
-  if (act == OGL_ACT_RELU) return z < 0.f ? 0.f : z;
-  if (act == OGL_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (act == OGL_ACT_GELU) return z * gn_phi(z, e);
-  return z;
+  if constexpr (ACT == OGL_ACT_RELU) return z < 0.f ? 0.f : z;
+  else if constexpr (ACT == OGL_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
+  else if constexpr (ACT == OGL_ACT_GELU) return z * gn_phi(z, e);
+  else return z;
 }
-__device__ __forceinline__ float gn_slope(float z, int act) {
-  if (act == OGL_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == OGL_ACT_SILU) {
+template <int ACT>
+__device__ __forceinline__ float gn_slope(float z) {
+  if constexpr (ACT == OGL_ACT_RELU) {
+    return z > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == OGL_ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     return s * __builtin_fmaf(z, 1.f - s, 1.f);
-  }
-  if (act == OGL_ACT_GELU) {
+  } else if constexpr (ACT == OGL_ACT_GELU) {
     float e;
     const float phi = gn_phi(z, e);
     return __builtin_fmaf(z * 0.39894228040143268f, e, phi);
+  } else {
+    return 1.f;
   }
-  return 1.f;
+}
+// f with the activation as a constant: one branch around a loop over many values instead of one at each of them
+template <typename F>
+__device__ __forceinline__ void gn_by_act(int act, F f) {
+  if (act == OGL_ACT_SILU) f(std::integral_constant<int, OGL_ACT_SILU>());
+  else if (act == OGL_ACT_GELU) f(std::integral_constant<int, OGL_ACT_GELU>());
+  else if (act == OGL_ACT_RELU) f(std::integral_constant<int, OGL_ACT_RELU>());
+  else f(std::integral_constant<int, OGL_ACT_NONE>());
 }
 
 // channel parameters c .. of a piece (`none` where there are none)
@@ -133,7 +146,7 @@ __device__ __forceinline__ float gn_block_sum(float v, float* lds) {
 // ================================================================ rows ========================================================================
 // One team per group and R rows one below the other; BLOCK: the team is the block.  NV pieces of V channels a lane and row.  R: a team's loads are
 // issued together; one piece a lane in flight leaves the memory waiting.
-template <typename T, int V, int NV, int R, bool BLOCK>
+template <typename T, int V, int NV, int R, bool BLOCK, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
   __shared__ float lds[4];
   const gn_team t(A, threadIdx.x & 63);
@@ -148,19 +161,19 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
   const int c0 = g * A.Cg;
   const T* xp = (const T*)A.x + (rows ? b : 0) * A.xb + c0;
   const bool tiny = A.Cg < V;
-  typename row_piece<T, V>::raw raw[R][NV];
+  typename PIECE::raw raw[R][NV];
   float v[R][NV][V], mean[R], rstd[R];
 #pragma unroll
   for (int q = 0; q < R; ++q)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int e0 = (j * lanes + lane) * V;
-      raw[q][j] = row_piece<T, V>(q < rows ? A.Cg - e0 : 0, tiny).fetch(xp + q * A.xb + e0);
+      raw[q][j] = PIECE(q < rows ? A.Cg - e0 : 0, tiny).fetch(xp + q * A.xb + e0);
     }
 #pragma unroll
   for (int q = 0; q < R; ++q)
 #pragma unroll
-    for (int j = 0; j < NV; ++j) row_piece<T, V>(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny).expand(raw[q][j], v[q][j]);
+    for (int j = 0; j < NV; ++j) PIECE(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny).expand(raw[q][j], v[q][j]);
   const float inv = 1.f / (float)A.Cg;
 #pragma unroll
   for (int q = 0; q < R; ++q) {
@@ -183,7 +196,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
           v[q][j][e] -= mean[q];
           d = __builtin_fmaf(v[q][j][e], v[q][j][e], d);
         }
-      } else if (n > 0) {
+      } else if (PIECE::cuts && n > 0) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           v[q][j][e] -= mean[q];
@@ -202,27 +215,29 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
       }
   }
   T* yp = (T*)A.y + b * A.yb + c0;
+  gn_by_act(A.act, [&](auto act) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int e0 = (j * lanes + lane) * V;
-    const row_piece<T, V> P(rows ? A.Cg - e0 : 0, tiny);
-    if (P.n <= 0) continue;
-    float w[V], bb[V];
-    gn_param<T, V>(A.w, A.p_type, c0 + e0, P, 1.f, w);
-    gn_param<T, V>(A.b, A.p_type, c0 + e0, P, 0.f, bb);
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = (j * lanes + lane) * V;
+      const PIECE P(rows ? A.Cg - e0 : 0, tiny);
+      if (P.n <= 0) continue;
+      float w[V], bb[V];
+      gn_param<T, V, PIECE>(A.w, A.p_type, c0 + e0, P, 1.f, w);
+      gn_param<T, V, PIECE>(A.b, A.p_type, c0 + e0, P, 0.f, bb);
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      if (q >= rows) continue;
+      for (int q = 0; q < R; ++q) {
+        if (q >= rows) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[q][j][e] = gn_act(__builtin_fmaf(v[q][j][e] * rstd[q], w[e], bb[e]), A.act);
-      P.store(yp + q * A.yb + e0, v[q][j], A.past);
+        for (int e = 0; e < V; ++e) v[q][j][e] = gn_act<decltype(act)::value>(__builtin_fmaf(v[q][j][e] * rstd[q], w[e], bb[e]));
+        P.store(yp + q * A.yb + e0, v[q][j], A.past);
+      }
     }
-  }
+  });
 }
 
 // A wave has tg groups side by side and rpw rows, a block its four waves' rows; block x of `chunks` takes every chunks-th set of rows, block y the next
 // groups.  The sums over its rows go to part[x][0: dz, 1: dz h][C].
-template <typename T, int V, int NV, int R, bool BLOCK>
+template <typename T, int V, int NV, int R, bool BLOCK, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
   __shared__ float lds[2 * GN_THREADS];
   const gn_team t(A, threadIdx.x & 63);
@@ -238,9 +253,9 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int e0 = (j * lanes + lane) * V;
-    const row_piece<T, V> P(mine ? A.Cg - e0 : 0, tiny);
-    gn_param<T, V>(A.w, A.p_type, c0 + e0, P, 1.f, w[j]);
-    gn_param<T, V>(A.b, A.p_type, c0 + e0, P, 0.f, bb[j]);
+    const PIECE P(mine ? A.Cg - e0 : 0, tiny);
+    gn_param<T, V, PIECE>(A.w, A.p_type, c0 + e0, P, 1.f, w[j]);
+    gn_param<T, V, PIECE>(A.b, A.p_type, c0 + e0, P, 0.f, bb[j]);
 #pragma unroll
     for (int e = 0; e < V; ++e) sz[j][e] = sh[j][e] = 0.f;
   }
@@ -252,7 +267,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
     const int64_t at = rows ? b : 0;
     const T* xp = (const T*)A.x + at * A.xb + c0;
     const T* gp = (const T*)A.dy + at * A.gb + c0;
-    typename row_piece<T, V>::raw rx[R][NV], rg[R][NV];
+    typename PIECE::raw rx[R][NV], rg[R][NV];
     float h[R][NV][V], dz[R][NV][V], mean[R], rstd[R], s1[R], s2[R];
 #pragma unroll
     for (int q = 0; q < R; ++q) {
@@ -261,7 +276,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int e0 = (j * lanes + lane) * V;
-        const row_piece<T, V> P(q < rows ? A.Cg - e0 : 0, tiny);
+        const PIECE P(q < rows ? A.Cg - e0 : 0, tiny);
         rx[q][j] = P.fetch(xp + q * A.xb + e0);
         rg[q][j] = P.fetch(gp + q * A.gb + e0);
       }
@@ -270,26 +285,28 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
     for (int q = 0; q < R; ++q)
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const row_piece<T, V> P(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny);
+        const PIECE P(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny);
         P.expand(rx[q][j], h[q][j]);
         P.expand(rg[q][j], dz[q][j]);
       }
+    gn_by_act(A.act, [&](auto act) {
 #pragma unroll
-    for (int q = 0; q < R; ++q) {
-      s1[q] = s2[q] = 0.f;
+      for (int q = 0; q < R; ++q) {
+        s1[q] = s2[q] = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)                                    // (behind a run's end dy is 0, and so is every term)
+        for (int j = 0; j < NV; ++j)                                  // (behind a run's end dy is 0, and so is every term)
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          h[q][j][e] = (h[q][j][e] - mean[q]) * rstd[q];
-          dz[q][j][e] *= gn_slope(__builtin_fmaf(h[q][j][e], w[j][e], bb[j][e]), A.act);
-          sz[j][e] += dz[q][j][e];
-          sh[j][e] = __builtin_fmaf(dz[q][j][e], h[q][j][e], sh[j][e]);
-          dz[q][j][e] *= w[j][e];
-          s1[q] += dz[q][j][e];
-          s2[q] = __builtin_fmaf(dz[q][j][e], h[q][j][e], s2[q]);
-        }
-    }
+          for (int e = 0; e < V; ++e) {
+            h[q][j][e] = (h[q][j][e] - mean[q]) * rstd[q];
+            dz[q][j][e] *= gn_slope<decltype(act)::value>(__builtin_fmaf(h[q][j][e], w[j][e], bb[j][e]));
+            sz[j][e] += dz[q][j][e];
+            sh[j][e] = __builtin_fmaf(dz[q][j][e], h[q][j][e], sh[j][e]);
+            dz[q][j][e] *= w[j][e];
+            s1[q] += dz[q][j][e];
+            s2[q] = __builtin_fmaf(dz[q][j][e], h[q][j][e], s2[q]);
+          }
+      }
+    });
     if (A.write_dx) {
 #pragma unroll
       for (int q = 0; q < R; ++q) {
@@ -303,7 +320,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
           const int e0 = (j * lanes + lane) * V;
-          const row_piece<T, V> P(q < rows ? A.Cg - e0 : 0, tiny);
+          const PIECE P(q < rows ? A.Cg - e0 : 0, tiny);
           if (P.n <= 0) continue;
 #pragma unroll
           for (int e = 0; e < V; ++e) dz[q][j][e] = __builtin_fmaf(dz[q][j][e], rstd[q], __builtin_fmaf(h[q][j][e], s2[q], s1[q]));
@@ -546,23 +563,25 @@ __device__ __forceinline__ void gn_apply_rows(const gn_args& A, const gn_place& 
       mu[e] = mean[g];
       a[e] *= rstd[g];
     }
-    for (int r = first; r < r1; r += U * step) {
-      raw_t raw[U];
+    gn_by_act(A.act, [&](auto act) {
+      for (int r = first; r < r1; r += U * step) {
+        raw_t raw[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (!WIDE && r == first) raw[u] = ahead[u];
-        else if (r + u * step < r1) raw[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
+        for (int u = 0; u < U; ++u) {
+          if (!WIDE && r == first) raw[u] = ahead[u];
+          else if (r + u * step < r1) raw[u] = C.fetch(xp + (int64_t)(r + u * step) * A.xl);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r + u * step >= r1) break;
+          float v[V];
+          C.expand(raw[u], v);
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[e] = gn_act<decltype(act)::value>(__builtin_fmaf(v[e] - mu[e], a[e], bb[e]));
+          C.store(yp + (int64_t)(r + u * step) * A.yl, v, A.past);
+        }
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (r + u * step >= r1) break;
-        float v[V];
-        C.expand(raw[u], v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = gn_act(__builtin_fmaf(v[e] - mu[e], a[e], bb[e]), A.act);
-        C.store(yp + (int64_t)(r + u * step) * A.yl, v, A.past);
-      }
-    }
+    });
   }
 }
 
@@ -671,7 +690,7 @@ __device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, c
 #pragma unroll
   for (int e = 0; e < V; ++e) sz[e] = sh[e] = 0.f;
   int r = r0;
-  auto rows = [&](auto count) {
+  auto rows = [&](auto count, auto act) {
     constexpr int U = decltype(count)::value;
     typename PIECE::raw rx[U], rg[U];
 #pragma unroll
@@ -687,15 +706,17 @@ __device__ __forceinline__ void gn_channel_sums(const gn_args& A, const T* xp, c
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float xm = v[e] - K.mu[e];
-        const float dz = d[e] * gn_slope(__builtin_fmaf(xm, K.a[e], K.b[e]), A.act);
+        const float dz = d[e] * gn_slope<decltype(act)::value>(__builtin_fmaf(xm, K.a[e], K.b[e]));
         sz[e] += dz;
         sh[e] = __builtin_fmaf(dz, xm, sh[e]);
       }
     }
     r += U * step;
   };
-  while (r + step < r1) rows(std::integral_constant<int, 2>());
-  while (r < r1) rows(std::integral_constant<int, 1>());
+  gn_by_act(A.act, [&](auto act) {
+    while (r + step < r1) rows(std::integral_constant<int, 2>(), act);
+    while (r < r1) rows(std::integral_constant<int, 1>(), act);
+  });
 #pragma unroll
   for (int e = 0; e < V; ++e) sh[e] *= K.rs[e];
 }
@@ -710,7 +731,7 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
     k2[e] = -K.rs[e] * K.rs[e] * s2[e];
   }
   int r = r0;
-  auto rows = [&](auto count) {
+  auto rows = [&](auto count, auto act) {
     constexpr int U = decltype(count)::value;
     typename PIECE::raw rx[U], rg[U];
 #pragma unroll
@@ -726,15 +747,17 @@ __device__ __forceinline__ void gn_dx_rows(const gn_args& A, const T* xp, const 
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float xm = v[e] - K.mu[e];
-        const float dz = d[e] * gn_slope(__builtin_fmaf(xm, K.a[e], K.b[e]), A.act);
+        const float dz = d[e] * gn_slope<decltype(act)::value>(__builtin_fmaf(xm, K.a[e], K.b[e]));
         v[e] = __builtin_fmaf(dz, K.a[e], __builtin_fmaf(xm, k2[e], k1[e]));
       }
       C.store(dp + (int64_t)(r + u * step) * A.yl, v, A.past);
     }
     r += U * step;
   };
-  while (r + step < r1) rows(std::integral_constant<int, 2>());
-  while (r < r1) rows(std::integral_constant<int, 1>());
+  gn_by_act(A.act, [&](auto act) {
+    while (r + step < r1) rows(std::integral_constant<int, 2>(), act);
+    while (r < r1) rows(std::integral_constant<int, 1>(), act);
+  });
 }
 
 // the window's channel sums over the block's positions -> out[0: dz, 1: dz h][C]; every thread takes part
@@ -991,7 +1014,7 @@ __global__ void __launch_bounds__(NT) k_gn_bwd_apply(gn_args A) {
 // ================================================================ host ========================================================================
 struct gn_plan {
   bool rows, block, wide;
-  bool even;                   // maps: every window is whole pieces
+  bool even;                   // every group (maps: window of groups) is whole pieces
   int threads;                 // maps: of a block
   int nv, r;                   // rows: pieces a lane, rows a team
   int64_t part, sums;          // floats of workspace
@@ -1019,6 +1042,7 @@ static gn_plan gn_make(gn_args& A, int x_type, bool backward) {
     // at most so many blocks: each leaves 2 C partial sums
     A.chunks = (int)std::min<int64_t>(ogl_cdiv(A.B, (P.block ? 1 : 4 * A.rpw) * P.r), std::max<int64_t>(1, 1024 / ogl_cdiv(A.G, A.tg)));
     A.by_lanes = ogl_div::make((uint32_t)A.lanes);
+    P.even = A.Cg % V == 0;
     A.by_tg = ogl_div::make((uint32_t)A.tg);
     P.part = backward ? (int64_t)A.chunks * 2 * A.C : 0;
     A.by_g = ogl_div::make((uint32_t)A.G);
@@ -1092,21 +1116,28 @@ extern "C" int64_t ogl_group_norm_workspace_bytes(int64_t B, int64_t L, int C, i
 template <typename T, int V>
 static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
   typedef row_piece<T, V> cut;
+  typedef row_even<T, V> even;
   typedef row_whole<T, V> whole;
   if (P.rows) {
     const int64_t grid = ogl_cdiv(ogl_cdiv(A.B, P.r) * A.G, P.block ? 1 : 4 * A.tw);
+#define GN_ROWS(NV, R, BLOCK)                                                  \
+  do {                                                                         \
+    if (P.even) GN_LAUNCH((k_gn_rows_fwd<T, V, NV, R, BLOCK, even>), grid);    \
+    else GN_LAUNCH((k_gn_rows_fwd<T, V, NV, R, BLOCK, cut>), grid);            \
+  } while (0)
     if (P.block) {
-      if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 1, true>), grid);
-      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 1, true>), grid);
-      else GN_LAUNCH((k_gn_rows_fwd<T, V, 4, 1, true>), grid);
+      if (P.nv == 1) GN_ROWS(1, 1, true);
+      else if (P.nv == 2) GN_ROWS(2, 1, true);
+      else GN_ROWS(4, 1, true);
     } else {
-      if (P.nv == 1 && P.r == 4) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 4, false>), grid);
-      else if (P.nv == 1) GN_LAUNCH((k_gn_rows_fwd<T, V, 1, 1, false>), grid);
-      else if (P.nv == 2 && P.r == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 2, false>), grid);
-      else if (P.nv == 2) GN_LAUNCH((k_gn_rows_fwd<T, V, 2, 1, false>), grid);
-      else if (P.nv == 3) GN_LAUNCH((k_gn_rows_fwd<T, V, 3, 1, false>), grid);
-      else GN_LAUNCH((k_gn_rows_fwd<T, V, 5, 1, false>), grid);
+      if (P.nv == 1 && P.r == 4) GN_ROWS(1, 4, false);
+      else if (P.nv == 1) GN_ROWS(1, 1, false);
+      else if (P.nv == 2 && P.r == 2) GN_ROWS(2, 2, false);
+      else if (P.nv == 2) GN_ROWS(2, 1, false);
+      else if (P.nv == 3) GN_ROWS(3, 1, false);
+      else GN_ROWS(5, 1, false);
     }
+#undef GN_ROWS
     return OGL_OK;
   }
   if (A.tiles == 1) {
@@ -1134,12 +1165,17 @@ static int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
 template <typename T, int V>
 static int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, hipStream_t st) {
   typedef row_piece<T, V> cut;
+  typedef row_even<T, V> even;
   typedef row_whole<T, V> whole;
   int64_t rows = 0, groups = 0;
   if (P.rows) {
     const dim3 grid((unsigned)A.chunks, (unsigned)ogl_cdiv(A.G, A.tg));
     if (grid.y > 65535) return OGL_EINVAL;
-#define GN_ROWS(NV, R, BLOCK) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK>), grid, dim3(GN_THREADS), 0, st, A)
+#define GN_ROWS(NV, R, BLOCK)                                                                                         \
+  do {                                                                                                                \
+    if (P.even) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK, even>), grid, dim3(GN_THREADS), 0, st, A);      \
+    else hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK, cut>), grid, dim3(GN_THREADS), 0, st, A);              \
+  } while (0)
     if (P.block) {
       if (P.nv == 1) GN_ROWS(1, 1, true);
       else if (P.nv == 2) GN_ROWS(2, 1, true);

@@ -40,6 +40,7 @@ template <typename T, int V>
 struct row_piece {
   static_assert(sizeof(T) * V == 16, "a piece is 16 bytes");
   typedef typename ogl_vec<T, V>::type raw;
+  static constexpr bool cuts = true;
   int n, back;
   bool tiny;
   __device__ __forceinline__ row_piece(int left, bool tiny_) : n(left), back(left > 0 && left < V && !tiny_ ? V - left : 0), tiny(tiny_) {}
@@ -75,16 +76,17 @@ struct row_piece {
   }
 };
 
-// The same where every run is a multiple of V: no ends to cut, so loads in a row have nothing between them.
+// The same where every run is a multiple of V: a piece is whole or (n <= 0) not there.
 template <typename T, int V>
-struct row_whole {
+struct row_even {
   typedef typename ogl_vec<T, V>::type raw;
-  static constexpr int n = V;
+  static constexpr bool cuts = false;
   static constexpr bool tiny = false;
-  __device__ __forceinline__ row_whole(int, bool) {}
+  int n;
+  __device__ __forceinline__ row_even(int left, bool) : n(left) {}
   __device__ __forceinline__ raw fetch(const T* __restrict__ p) const {
-    raw t;
-    __builtin_memcpy(&t, p, 16);
+    raw t = (raw)(T)0.f;
+    if (n > 0) __builtin_memcpy(&t, p, 16);
     return t;
   }
   __device__ __forceinline__ void expand(raw t, float (&v)[V]) const {
@@ -93,9 +95,16 @@ struct row_whole {
   }
   __device__ __forceinline__ void load(const T* __restrict__ p, float (&v)[V]) const { expand(fetch(p), v); }
   __device__ __forceinline__ void store(T* __restrict__ p, const float (&v)[V], bool past) const {
+    if (n <= 0) return;
     if (past) row_store_nt<T, V>(p, v);
     else row_store<T, V>(p, v);
   }
+};
+// And where the caller has asked already: loads in a row have nothing between them.
+template <typename T, int V>
+struct row_whole : row_even<T, V> {
+  static constexpr int n = V;
+  __device__ __forceinline__ row_whole(int, bool) : row_even<T, V>(V, false) {}
 };
 
 // n / d for 0 <= n < 2^31 and 1 <= d < 2^31 as a multiplication: m = ceil(2^(31 + s) / d) with 2^s >= d, so m d = 2^(31 + s) + e, e < d <= 2^s,

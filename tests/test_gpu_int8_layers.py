@@ -136,7 +136,7 @@ def test_rows_of_large_outputs(ops, width):
 
 
 def test_map_of_large_outputs(ops):
-    """1200 samples, one block each, of 36 x 36 x 24 in float32 (149 MB): the same bits sample by sample group as in halves that are also that many."""
+    """2400 samples of 30 x 384, a block each whatever their number: the same bits in halves too small for it."""
     gen = torch.Generator(device="cuda").manual_seed(0)
     x = torch.randn(2400, 30, 24 * 16, device="cuda", generator=gen)                   # 110 MB; halves of 55 MB
     y = ops.group_norm(x, 4, activation="silu")

@@ -118,6 +118,14 @@ def test_linear_c_entry_checks_its_arguments():
     assert call(M=0) == 0 and call(N=0) == 0
 
 
+def test_linear_c_entry_refuses_tables_beyond_its_offsets():
+    h = _lib.lib()
+    buf = (ctypes.c_char * 4096)()
+    p = (ctypes.addressof(buf) + 63) // 64 * 64
+    for nrows, ldx, n, ldw in [(2 ** 32, 64, 6, 64), (4, 2 ** 37, 6, 64), (2 ** 20, 2 ** 18, 6, 64), (4, 64, 2 ** 30, 256), (4, 64, 6, 2 ** 36)]:
+        assert h.ogl_linear_i8(p, ldx, p, None, nrows, 3, 40, p, ldw, p, n, None, 0, p, n, 0, None) == -1
+
+
 def test_group_norm_refuses():
     x = torch.zeros(4, 12)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
