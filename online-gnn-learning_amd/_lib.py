@@ -132,6 +132,10 @@ SIGNATURES = {
     "ogl_sample_blocks_small_fill": (_i, [_p, _p, _p, _i, _i, C.c_uint64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p]),
     "ogl_stage_segments": (_i, [_i, _p, _p, _p, _p, _p, _i64, _p]),
     "ogl_fuse_block_segments": (_i, [_p, _p, _i, _p, _p, _i, _p, _p]),
+}
+
+# include/ogl_rows.h, one to one
+ROW_SIGNATURES = {
     "ogl_quant_rows_workspace_bytes": (_i64, [_i64, _i64, _i]),
     "ogl_quant_rows_write": (_i, [_p, _i64, _i, _i64, _i, _p, _i64, _p, _i64, _i, _p, _i64, _i, _p, _i64, _p]),
     "ogl_group_norm_workspace_bytes": (_i64, [_i64, _i64, _i, _i, _i, _i]),
@@ -165,7 +169,7 @@ def lib():
                 "(hipcc --offload-arch=gfx950).  There is no CPU fallback." % LIB_PATH)
         import torch  # noqa: F401  (loads torch's libamdhip64.so.7 first; ours binds to the same SONAME)
         h = C.CDLL(LIB_PATH, mode=C.RTLD_GLOBAL)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (*SIGNATURES.items(), *ROW_SIGNATURES.items()):
             fn = getattr(h, name)   # AttributeError here = header/library drift
             fn.restype = res
             fn.argtypes = args

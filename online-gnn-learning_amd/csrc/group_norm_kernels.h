@@ -151,18 +151,6 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
   for (int q = 0; q < R; ++q)
 #pragma unroll
     for (int j = 0; j < NV; ++j) PIECE(q < rows ? A.Cg - (j * lanes + lane) * V : 0, tiny).expand(raw[q][j], v[q][j]);
-  // (the parameters of one or two pieces as well: behind the reductions their loads would be waited for)
-  constexpr bool EARLY = NV <= 2;
-  float w[NV][V], bb[NV][V];
-  auto params = [&](int j) {
-    const int e0 = (j * lanes + lane) * V;
-    const PIECE P(rows ? A.Cg - e0 : 0, tiny);
-    gn_param<T, V, PIECE>(A.w, A.p_type, c0 + e0, P, 1.f, w[j]);
-    gn_param<T, V, PIECE>(A.b, A.p_type, c0 + e0, P, 0.f, bb[j]);
-  };
-  if (EARLY)
-#pragma unroll
-    for (int j = 0; j < NV; ++j) params(j);
   const float inv = 1.f / (float)A.Cg;
 #pragma unroll
   for (int q = 0; q < R; ++q) {
@@ -210,12 +198,14 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
       const int e0 = (j * lanes + lane) * V;
       const PIECE P(rows ? A.Cg - e0 : 0, tiny);
       if (P.n <= 0) continue;
-      if (!EARLY) params(j);
+      float w[V], bb[V];                                               // (loaded ahead of the reductions they cost registers and time: 64 -> 70 us)
+      gn_param<T, V, PIECE>(A.w, A.p_type, c0 + e0, P, 1.f, w);
+      gn_param<T, V, PIECE>(A.b, A.p_type, c0 + e0, P, 0.f, bb);
 #pragma unroll
       for (int q = 0; q < R; ++q) {
         if (q >= rows) continue;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[q][j][e] = gn_act<decltype(act)::value>(__builtin_fmaf(v[q][j][e] * rstd[q], w[j][e], bb[j][e]));
+        for (int e = 0; e < V; ++e) v[q][j][e] = gn_act<decltype(act)::value>(__builtin_fmaf(v[q][j][e] * rstd[q], w[e], bb[e]));
         P.store(yp + q * A.yb + e0, v[q][j], A.past);
       }
     }

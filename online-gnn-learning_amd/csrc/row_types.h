@@ -3,6 +3,7 @@
 // row such as 602 floats starts at any multiple of 8 bytes, so a 16-byte access is one instruction wherever it falls.
 #pragma once
 #include "ogl_common.h"
+#include "ogl_rows.h"
 
 typedef __bf16 ogl_bf16;
 typedef _Float16 ogl_f16;

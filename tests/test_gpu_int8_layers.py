@@ -361,6 +361,37 @@ def test_train_steps_with_a_norm_captured_and_eager(ops):
     np.testing.assert_allclose([l for _, l in losses[True]], [l for _, l in losses[False]], rtol=2e-4)
 
 
+def test_every_row_entry_point_is_reached(ops):
+    """Training with a norm, evaluation on quantised features and a cache written by ids call every symbol of include/ogl_rows.h."""
+    from ogl_amd import _lib, sampling
+    from ogl_amd.graphsage import GatheredRows, GraphSAGE, GroupNorm
+    from ogl_amd.graphsage.model import RandomHipSupervisedGraphSage
+    ops._norm_workspace.cache_clear()
+    real, seen = _lib.lib(), set()
+
+    class Proxy:
+        def __getattr__(self, name):
+            seen.add(name)
+            return getattr(real, name)
+    _lib._lib = Proxy()
+    try:
+        feat_size, labels, dyn, n_classes = toy()
+        g = dyn.get_graph()
+        model = GraphSAGE(feat_size, 16, n_classes, 1, None, 0, "pool", edge_feats=0, norm=lambda width: GroupNorm(4, width, activation="relu")).cuda()
+        st = RandomHipSupervisedGraphSage(model, 1, 16, labels, 5, cuda=True, batch_full=32)
+        st.use_graphs, st.quantize_features = False, True
+        st.build_optimizer()
+        st._train_batches(g, np.arange(16), 16)
+        st._run_custom_eval(g, None, None, np.arange(g.n_present))
+        cache = ops.quant_rows(40, feat_size)
+        ids = torch.arange(300, device="cuda") % 40
+        ops.quant_rows_write(cache, g.ndata["feat"][:1].expand(300, -1), slots=ids)
+        GatheredRows(cache, ids).materialize()
+    finally:
+        _lib._lib = real
+    assert set(_lib.ROW_SIGNATURES) <= seen, set(_lib.ROW_SIGNATURES) - seen
+
+
 # ---- custom ops -----------------------------------------------------------------------------------------------------------------------------------
 def test_custom_ops(ops):
     import ogl_amd.torch_ops  # noqa: F401

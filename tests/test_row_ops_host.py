@@ -1,5 +1,7 @@
 """The row operators refuse what they cannot do, before anything reaches a GPU."""
 import ctypes
+import os
+import re
 
 import pytest
 import torch
@@ -10,6 +12,18 @@ from ogl_amd import _lib, ops
 
 def cache(n=4, width=40, group=None, fmt="int8"):
     return ops.quant_rows(n, width, group, fmt, device="cpu")
+
+
+def test_header_symbols_exported_and_bound():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {}
+    for header in ("ogl_hip.h", "ogl_rows.h"):
+        src = re.sub(r"/\*.*?\*/", "", open(os.path.join(root, "include", header)).read(), flags=re.S)
+        names[header] = set(re.findall(r"\b(ogl_[a-z0-9_]+)\s*\(", src))
+    assert names["ogl_rows.h"] == set(_lib.ROW_SIGNATURES) and not names["ogl_rows.h"] & names["ogl_hip.h"]
+    h = _lib.lib()
+    for n in names["ogl_rows.h"]:
+        assert getattr(h, n).argtypes == _lib.ROW_SIGNATURES[n][1]
 
 
 def test_quant_rows_layout():
