@@ -394,7 +394,7 @@ class HipSupervisedGraphSage(SupervisedGraphSage):
     # intermediate: the products run as several rounds of tiles instead of a fraction of one
     FUSE_INFERENCE_ROWS = 131072
     # the per-pass tables from features kept in 8 bits (SnapshotGraph.quantized_features) and weights quantised for the pass: about 0.4 % of a
-    # row's largest feature off, at 8-bit matrix rate (opt-in: float32 tables otherwise)
+    # row's largest feature off, at 8-bit matrix rate (opt-in: float32 tables otherwise; layers without a pooling projection have no such tables)
     quantize_features = False
 
     def _projection_tables(self, graph, layer0):

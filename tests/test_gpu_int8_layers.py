@@ -144,6 +144,48 @@ def test_map_of_large_outputs(ops):
         assert torch.equal(y[s], ops.group_norm(x[s], 4, activation="silu"))
 
 
+# ---- offsets that pass 32 bits --------------------------------------------------------------------------------------------------------------------
+def test_products_and_reads_behind_four_gigabytes(ops):
+    """Rows of a table of 4.4 GB: the same bits as from a small table that holds the same rows."""
+    n, w, k = 4_300_000, 1000, 64
+    gen = torch.Generator().manual_seed(0)
+    small = ops.quantize_rows(torch.randn(k, w, generator=gen).cuda())
+    at = torch.randint(0, n, (k,), generator=gen)
+    at[0], at[1], at[2] = n - 1, 2 ** 32 // 1024, 2 ** 31 // 1024
+    at = torch.unique(at)
+    table = ops.quant_rows(n, w)
+    table.codes[at.cuda()], table.scales[at.cuda()] = small.codes[:len(at)], small.scales[:len(at)]
+    weight = ops.quantize_rows(torch.randn(70, w, generator=gen).cuda())
+    for m in (5, 60, 300, 9000):
+        pick = torch.randint(0, len(at), (m,), generator=gen)
+        far, near = at[pick].cuda(), pick.cuda()
+        assert torch.equal(ops.linear_int8(table, weight, x_rows=far), ops.linear_int8(small, weight, x_rows=near))
+        assert torch.equal(ops.quant_rows_read(table, far), ops.quant_rows_read(small, near))
+    wide = ops.quantize_rows(torch.randn(9000, w, generator=gen).cuda())                 # (large tiles of the product)
+    pick = torch.randint(0, len(at), (9000,), generator=gen)
+    assert torch.equal(ops.linear_int8(table, wide, x_rows=at[pick].cuda()), ops.linear_int8(small, wide, x_rows=pick.cuda()))
+
+
+def test_norm_behind_four_gigabytes(ops):
+    """Rows and samples whose offsets pass 2^31 elements: the same bits as in a call on the last of them alone."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    w, b = torch.rand(1000, device="cuda", generator=gen), torch.rand(1000, device="cuda", generator=gen)
+    x = torch.randn(2_300_000, 1000, device="cuda", generator=gen, dtype=torch.bfloat16)
+    y, stats = ops.group_norm_fwd(x, 4, w, b, 1e-5, 2, True)
+    dx = ops.group_norm_bwd(x, x, 4, w, b, stats, 2)[0]
+    last = slice(2_200_000, None)
+    y1, st1 = ops.group_norm_fwd(x[last], 4, w, b, 1e-5, 2, True)
+    assert torch.equal(y[last], y1) and torch.equal(stats[:, last], st1)
+    assert torch.equal(dx[last], ops.group_norm_bwd(x[last], x[last], 4, w, b, st1, 2)[0])
+    x = x[:2_200_000].view(1100, 2000, 1000)
+    y, stats = ops.group_norm_fwd(x, 4, w, b, 1e-5, 2, True)
+    dx = ops.group_norm_bwd(x, x, 4, w, b, stats, 2)[0]
+    last = slice(70, None)
+    y1, st1 = ops.group_norm_fwd(x[last], 4, w, b, 1e-5, 2, True)
+    assert torch.equal(y[last], y1) and torch.equal(stats[:, last], st1)
+    assert torch.equal(dx[last], ops.group_norm_bwd(x[last], x[last], 4, w, b, st1, 2)[0])
+
+
 # ---- products of middle size ----------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("M,N,K,gather", [(2001, 1700, 1100, False), (300, 12200, 1030, True), (1537, 2049, 1024, True)])
