@@ -5,7 +5,7 @@
 // sx sw, their product, and the addition of the bias.
 //
 // Both operands lie K-contiguous (a weight's rows are its output channels), which is what the matrix instruction reads: 16 bytes of one row a lane.
-// Rows are a multiple of 64 bytes with zeros behind the last column, so there is no tail in K beyond a missing half step.  The weight rows are the
+// Rows are a multiple of 64 bytes with zeros behind the last column, so there is no tail in K.  The weight rows are the
 // instruction's first operand: a lane then holds 4 consecutive output columns of one row of y, a 16-byte store.
 #include <algorithm>
 #include "row_types.h"
@@ -77,7 +77,9 @@ __device__ __forceinline__ void i8_out(const i8_args& A, int64_t m, int n, v4i32
 }
 
 // ---- few rows: every wave of a block takes a slice of K for the block's 16 output columns, straight from memory to the matrix unit ----------------
-// 16 weight rows x K a block, so N / 16 blocks; the weight is read once per MT * 16 rows of x and bounds the time.
+// 16 weight rows x K a block, so N / 16 blocks; the weight is read once per MT * 16 rows of x and bounds the time: 16 x 12288, K = 4096 takes 14.5 us,
+// 3.5 TB/s of a weight that no cache holds (two steps a lane side by side, eight of them in flight, 4 or 16 waves and loads past the caches: the same
+// or slower).
 template <typename T, int MT>
 __global__ void __launch_bounds__(512) k_i8_few(i8_args A) {
   constexpr int WAVES = 8;
@@ -397,7 +399,9 @@ static int i8_launch(const i8_args& A, hipStream_t st) {
     hipLaunchKernelGGL((k_i8_few<T, 1>), dim3(nb, 1), dim3(512), 0, st, A);
     return OGL_OK;
   }
-  if (A.M <= 64) {
+  // Up to 64 rows while the blocks of 16 columns fit one a CU: behind that they read x as often as w.  32 x 4096, K = 4096: 11.7 us, in tiles 12.5 us;
+  // 32 x 6144 16.2 us, 12.6 us; 64 x 12288 30.7 us, 14.4 us; 64 x 600, K = 602 4.4 us, 5.4 us.
+  if (A.M <= 64 && nb <= 256) {
     hipLaunchKernelGGL((k_i8_few<T, 4>), dim3(nb, 1), dim3(512), 0, st, A);
     return OGL_OK;
   }

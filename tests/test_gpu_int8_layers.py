@@ -209,6 +209,20 @@ def test_linear_of_middle_size(ops, dtype, M, N, K, gather):
     assert ((got.double() - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("M", [16, 17, 33, 64, 65])
+@pytest.mark.parametrize("N", [4090, 4100])
+def test_linear_of_few_rows_and_many_columns(ops, M, N):
+    """Exact sums in every form, so the same bits as rows of a product that takes another one (as many rows as its tiles ask for)."""
+    gen = torch.Generator().manual_seed(M)
+    x, w = ops.quantize_rows(torch.randn(300, 333, generator=gen).cuda()), ops.quantize_rows(torch.randn(N, 333, generator=gen).cuda())
+    bias = torch.randn(N, generator=gen).cuda()
+    whole = ops.linear_int8(x, w, bias, True)
+    assert torch.equal(ops.linear_int8(x, w, bias, True, torch.arange(M, device="cuda")), whole[:M])
+    p = x.codes[:M, :333].double() @ w.codes[:, :333].double().t() * x.scales[:M].double() * w.scales.double().t()
+    want = (p + bias.double()).clamp(min=0)
+    assert ((whole[:M].double() - want).abs() <= 2.0 ** -24 * (5 * p.abs() + bias.double().abs())).all()
+
+
 def test_linear_into_a_given_matrix(ops):
     gen = torch.Generator().manual_seed(1)
     x, w = ops.quantize_rows(torch.randn(200, 100, generator=gen).cuda()), ops.quantize_rows(torch.randn(70, 100, generator=gen).cuda())
