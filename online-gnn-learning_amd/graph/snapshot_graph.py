@@ -8,6 +8,8 @@ the reference's ``graph.ndata['feat'] / ['target']`` contract as views of reside
 """
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import torch
 
@@ -39,6 +41,14 @@ def build_time_ordered_csr(n, src, dst, key):
     return indptr, indices, keys
 
 
+class _QuantizedFeatures:
+    """What the views of one stream share of ``quantized_features``: the table, how many of its rows are written, the stream it was allocated on."""
+
+    def __init__(self):
+        self.lock = threading.Lock()
+        self.rows, self.written, self.stream = None, 0, None
+
+
 class SnapshotGraph:
     """What the hot path needs of a graph: the sampler handle, ``ndata`` and the node count."""
 
@@ -61,7 +71,7 @@ class SnapshotGraph:
         target = torch.as_tensor(np.asarray(target)).reshape(n, -1)[:, :1].to(torch.int64)
         self.target_table = target.to(self.device).contiguous()
         self.edata = {}
-        self._quantized = {}
+        self._quantized = _QuantizedFeatures()
         self.n_present = 0
         self.cut = 0
         self.ndata = {"feat": self.feat_table[:0], "target": self.target_table[:0]}
@@ -91,17 +101,26 @@ class SnapshotGraph:
 
     def quantized_features(self):
         """The present vertices' feature rows in 8 bits (``ops.QuantRows``, int8, one scale a row).  Each row is quantised once, when a call first
-        finds it present: features are static, so the cache only grows with the stream (shared by the views of one stream)."""
-        q = self._quantized
-        if "rows" not in q:
-            q["rows"], q["written"] = ops.quant_rows(self.n_total, self.feat_table.shape[1], device=self.device), 0
-        rows, done = q["rows"], q["written"]
-        if done < self.n_present:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("quantized_features: rows %d .. %d are new, call it once before the capture" % (done, self.n_present))
-            ops.quant_rows_write(rows, self.feat_table[done:self.n_present], start=done)
-            q["written"] = self.n_present
-        n = self.n_present
+        finds it present: features are static, so the cache only grows with the stream (shared by the views of one stream).  A call that adds
+        rows returns when they are written (the only wait for the device here), so that a later call finds them there, whichever stream,
+        thread or view it comes from."""
+        q, dev, n = self._quantized, self.feat_table.device, self.n_present
+        with q.lock, torch.cuda.device(dev):
+            stream = torch.cuda.current_stream(dev)
+            fresh = q.rows is None
+            if fresh:
+                q.rows, q.stream = ops.quant_rows(self.n_total, self.feat_table.shape[1], device=dev), stream
+            if q.written < n:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("quantized_features: rows %d .. %d are new, call it once before the capture" % (q.written, n))
+                ops.quant_rows_write(q.rows, self.feat_table[q.written:n], start=q.written)
+            if q.written < n or fresh:
+                stream.synchronize()
+                q.written = n
+            rows = q.rows
+            if stream != q.stream and not torch.cuda.is_current_stream_capturing():
+                rows.codes.record_stream(stream)                        # (freed memory is not handed out while this stream may read it)
+                rows.scales.record_stream(stream)
         return ops.QuantRows(rows.codes[:n], rows.scales[:n], rows.width)
 
     def number_of_nodes(self):
