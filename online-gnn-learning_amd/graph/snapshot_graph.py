@@ -106,19 +106,20 @@ class SnapshotGraph:
         thread or view it comes from."""
         q, dev, n = self._quantized, self.feat_table.device, self.n_present
         with q.lock, torch.cuda.device(dev):
-            stream = torch.cuda.current_stream(dev)
-            fresh = q.rows is None
-            if fresh:
-                q.rows, q.stream = ops.quant_rows(self.n_total, self.feat_table.shape[1], device=dev), stream
+            stream, capturing = torch.cuda.current_stream(dev), torch.cuda.is_current_stream_capturing()
             if q.written < n:
-                if torch.cuda.is_current_stream_capturing():
+                # (refused before anything is allocated: the zero fill of a table from a graph's own memory would run at every replay)
+                if capturing:
                     raise RuntimeError("quantized_features: rows %d .. %d are new, call it once before the capture" % (q.written, n))
-                ops.quant_rows_write(q.rows, self.feat_table[q.written:n], start=q.written)
-            if q.written < n or fresh:
+                rows = q.rows if q.rows is not None else ops.quant_rows(self.n_total, self.feat_table.shape[1], device=dev)
+                ops.quant_rows_write(rows, self.feat_table[q.written:n], start=q.written)
                 stream.synchronize()
-                q.written = n
+                q.stream = stream if q.rows is None else q.stream
+                q.rows, q.written = rows, n
+            if q.rows is None:
+                return ops.quant_rows(0, self.feat_table.shape[1], device=dev)
             rows = q.rows
-            if stream != q.stream and not torch.cuda.is_current_stream_capturing():
+            if stream != q.stream and not capturing:
                 rows.codes.record_stream(stream)                        # (freed memory is not handed out while this stream may read it)
                 rows.scales.record_stream(stream)
         return ops.QuantRows(rows.codes[:n], rows.scales[:n], rows.width)

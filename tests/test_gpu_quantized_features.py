@@ -45,3 +45,29 @@ def test_two_streams_share_the_table(ops):
         torch.cuda.synchronize()
         assert torch.equal(codes, want.codes[:present]) and torch.equal(scales, want.scales[:present])
         del busy
+
+
+def test_captured_after_the_rows_are_there(ops):
+    """A first call inside a capture is refused; after one outside it, the rows are read by every replay, with eager work in between."""
+    g = toy()
+    n, cut = g.n_present, g.cut
+    at = torch.arange(0, n, 2, device="cuda")
+    x = torch.zeros(n, 8, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):                                           # (it records the caller's own work all the same)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            g.quantized_features()
+        y = x + 1
+    graph.replay()
+    want = ops.quant_rows_read(g.quantized_features(), at)
+    graph.replay()
+    assert torch.equal(ops.quant_rows_read(g.quantized_features(), at), want) and float(want.abs().max()) > 0
+    second = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(second):
+        z = ops.quant_rows_read(g.quantized_features(), at)
+    for step in range(3):
+        z.zero_()
+        second.replay()
+        graph.replay()
+        assert torch.equal(z, want) and (y == 1).all()
+        assert torch.equal(ops.quant_rows_read(g.quantized_features(), at), want)

@@ -26,7 +26,7 @@ class Device:
             @staticmethod
             def quant_rows(n, width, **kw):
                 time.sleep(0.02)                                        # (another thread gets its turn here)
-                dev.queued.append("zeros")
+                dev.queued += ["zeros"] * (n > 0)
                 return real_ops.quant_rows(n, width, device="cpu")
 
             @staticmethod
@@ -106,3 +106,24 @@ def test_two_threads_make_one_table(monkeypatch):
     for t in threads:
         t.join()
     assert dev.written == ["zeros", (0, N)] and got[0].codes.data_ptr() == got[1].codes.data_ptr()
+
+
+@pytest.mark.parametrize("present", [0, 5])
+def test_a_first_call_inside_a_capture_keeps_nothing(monkeypatch, present):
+    """A table allocated there would live in the graph's memory, its zero fill a node of the graph: cleared again at every replay."""
+    dev = Device(monkeypatch)
+    dev.capturing = True
+    g = graph(present)
+    if present:
+        with pytest.raises(RuntimeError, match="before the capture"):
+            g.quantized_features()
+    else:
+        assert g.quantized_features().n == 0
+    assert g._quantized.rows is None and g._quantized.written == 0 and (0, present) not in dev.queued
+    dev.capturing = False
+    dev.queued.clear()
+    assert view(g, N).quantized_features().n == N and dev.written == ["zeros", (0, N)]
+    dev.capturing = True
+    assert g.quantized_features().n == present and dev.queued == []
+    g.n_present = N
+    assert g.quantized_features().n == N
