@@ -13,6 +13,7 @@ import os
 import weakref
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import REDUCE_OPS, check
@@ -3291,6 +3292,14 @@ def _row_device(what, first, *others):
     return dev
 
 
+def _row_no_tangents(what, *tensors):
+    """Raises for a tensor with a forward-mode tangent (outside a dual level there is none): the kernels would drop it."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("%s has no forward-mode derivative" % what)
+
+
 def _row_launch(dev, name, fn, *args, **meta):
     """``_launch`` on ``dev``'s current stream, whichever device is current."""
     index = dev.index
@@ -3453,6 +3462,7 @@ def linear_int8(x, w, bias=None, relu=False, x_rows=None, dtype=torch.float32, o
         raise ValueError("%s: float32, bfloat16 or float16 results, not %s" % (what, dtype))
     if torch.is_grad_enabled() and ((isinstance(x, torch.Tensor) and x.requires_grad) or (bias is not None and bias.requires_grad)):
         raise RuntimeError("%s is inference only (run it under torch.no_grad())" % what)
+    _row_no_tangents(what, x, bias)
     if isinstance(x, torch.Tensor):
         if x_rows is not None:
             raise ValueError("%s: x_rows selects rows of a QuantRows" % what)
@@ -3589,7 +3599,7 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None)
     """``act(group_norm(x) * weight + bias)``, channels LAST: ``x`` [B, *spatial, C] in float32 / bfloat16 / float16, statistics over the positions of
     a sample and the C / num_groups channels of a group (a matrix [n, C]: over the channels of its row).  ``weight`` / ``bias`` [C] of the type of x
     or float32; ``activation`` None, 'relu', 'silu' or 'gelu' (x Phi(x)).  Statistics and sums are float32, each result is rounded once.
-    Differentiable (once) w.r.t. x, weight and bias; results do not depend on the run (no atomics)."""
+    Differentiable (once, in reverse mode) w.r.t. x, weight and bias; results do not depend on the run (no atomics)."""
     what = "group_norm"
     if x.dim() < 2:
         raise ValueError("%s: expected [B, *spatial, C], got shape %s" % (what, tuple(x.shape)))
@@ -3607,6 +3617,7 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None)
             raise ValueError("%s: weight and bias must be contiguous [%d] of float32 or %s" % (what, C, x.dtype))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("%s: weight and bias of different types" % what)
+    _row_no_tangents(what, x, weight, bias)
     _row_device(what, x, weight, bias)
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
