@@ -212,8 +212,8 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_fwd(gn_args A) {
   });
 }
 
-// A wave has tg groups side by side and rpw rows, a block its four waves' rows; block x of `chunks` takes every chunks-th set of rows, block y the next
-// groups.  The sums over its rows go to part[x][0: dz, 1: dz h][C].
+// A wave has tg groups side by side and rpw rows, a block its four waves' rows; block x of `chunks` takes every chunks-th set of rows, blocks (y, z) the
+// next groups.  The sums over its rows go to part[x][0: dz, 1: dz h][C].
 template <typename T, int V, int NV, int R, bool BLOCK, typename PIECE>
 __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
   __shared__ float lds[2 * GN_THREADS];
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(GN_THREADS) k_gn_rows_bwd(gn_args A) {
   const int lanes = BLOCK ? GN_THREADS : A.lanes, lane = BLOCK ? (int)threadIdx.x : t.pos;
   const int rw = BLOCK ? 0 : (int)A.by_tg.div((uint32_t)t.team), gi = BLOCK ? 0 : t.team - rw * A.tg;
   const int ri = BLOCK ? 0 : (int)(threadIdx.x >> 6) * A.rpw + rw, block_rows = BLOCK ? 1 : 4 * A.rpw;
-  const int g = blockIdx.y * A.tg + gi;
+  const int g = (blockIdx.z * gridDim.y + blockIdx.y) * A.tg + gi;
   const bool mine = g < A.G && (BLOCK || (t.on && rw < A.rpw));
   const int c0 = (mine ? g : 0) * A.Cg;
   const float inv = 1.f / (float)A.Cg;
@@ -1053,8 +1053,8 @@ int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, hipStrea
   typedef row_whole<T, V> whole;
   int64_t rows = 0, groups = 0;
   if (P.rows) {
-    const dim3 grid((unsigned)A.chunks, (unsigned)ogl_cdiv(A.G, A.tg));
-    if (grid.y > 65535) return OGL_EINVAL;
+    const int64_t sets = ogl_cdiv(A.G, A.tg), z = ogl_cdiv(sets, 65535);   // (a launch's y ends at 65535: 2^22 groups of one channel are 65536 sets)
+    const dim3 grid((unsigned)A.chunks, (unsigned)ogl_cdiv(sets, z), (unsigned)z);
 #define GN_ROWS(NV, R, BLOCK)                                                                                         \
   do {                                                                                                                \
     if (P.even) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK, even>), grid, dim3(GN_THREADS), 0, st, A);      \
