@@ -2,7 +2,7 @@
 //
 // The sum is exact (int32 accumulators of v_mfma_i32_32x32x32_i8 and 16x16x64; |sum| <= 128^2 K < 2^31 for K < 131072, whatever the bytes hold), so its
 // order is free: waves may split K and partial sums may be joined in any order with the same result.  Rounded to float32: the sum once (above 2^24),
-// sx sw, their product, and the addition of the bias.
+// sx sw, and, in one fused step, their product with the bias added; every form does the same, so a row's bits do not depend on the form.
 //
 // Both operands lie K-contiguous (a weight's rows are its output channels), which is what the matrix instruction reads: 16 bytes of one row a lane.
 // Rows are a multiple of 64 bytes with zeros behind the last column, so there is no tail in K.  The weight rows are the
@@ -58,7 +58,7 @@ __device__ __forceinline__ void i8_columns(const i8_args& A, int n, float (&sw)[
 __device__ __forceinline__ void i8_values(const i8_args& A, v4i32 acc, float sx, const float (&sw)[4], const float (&b)[4], float (&v)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    v[i] = (float)acc[i] * (sx * sw[i]) + b[i];
+    v[i] = __builtin_fmaf((float)acc[i], sx * sw[i], b[i]);
     if (A.relu) v[i] = v[i] < 0.f ? 0.f : v[i];                     // (a NaN stays)
   }
 }
