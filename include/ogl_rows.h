@@ -35,7 +35,8 @@ int ogl_quant_rows_read(const void* codes, int64_t ldc, int format, const float*
 /* y[m, n] = act((sx[r] sw[n]) * sum_k x[r, k] w[n, k] + bias[n]), r = rows[m] (NULL: m, then M <= nrows): the product of two caches in int8 with
  * one scale a row (a weight's rows are its output channels), act = relu or none, y in y_type.  The sum is exact; everything behind it is float32.
  * x [nrows, ldx], w [N, ldw]: 64-byte aligned, ld a multiple of 64, zeros behind column K in at least one of them; 1 <= K < 131072.
- * Rows outside [0, nrows) count as zero rows (y = act(bias)).  Tables of 2^38 bytes and more: OGL_EINVAL. */
+ * Rows outside [0, nrows) count as zero rows (y = act(bias); NaN where a weight's scale is).  Tables of 2^38 bytes and more, an empty table (nrows = 0
+ * with M > 0), N of 2^31 - 256 and more (with M <= 16: 2^27 - 15 and more, the launch's threads): OGL_EINVAL. */
 int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const int64_t* rows, int64_t nrows, int64_t M, int K, const void* w, int64_t ldw,
                   const float* sw, int N, const float* bias, int relu, void* y, int64_t ldy, int y_type, ogl_stream_t stream);
 

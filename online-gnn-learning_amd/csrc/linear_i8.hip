@@ -396,6 +396,7 @@ template <typename T>
 static int i8_launch(const i8_args& A, hipStream_t st) {
   const unsigned nb = (unsigned)ogl_cdiv(A.N, 16);
   if (A.M <= 16) {
+    if ((int64_t)nb * 512 > (int64_t)UINT32_MAX) return OGL_EINVAL;   // the launch has at most 2^32 - 1 threads
     hipLaunchKernelGGL((k_i8_few<T, 1>), dim3(nb, 1), dim3(512), 0, st, A);
     return OGL_OK;
   }
@@ -419,6 +420,7 @@ extern "C" int ogl_linear_i8(const void* x, int64_t ldx, const float* sx, const 
   if (M < 0 || N < 0 || K < 1 || K > 131071 || nrows < 0 || ldx < K || ldw < K || ldx % 64 || ldw % 64 || ldy < N || y_type < OGL_F32 || y_type > OGL_F16)
     return OGL_EINVAL;
   if (!rows && M > nrows) return OGL_EINVAL;
+  if (N > INT32_MAX - 256) return OGL_EINVAL;                           // (columns of a whole tile are counted in 31 bits)
   const double most = 4294967296.;                                    // offsets count 64 bytes in 32 bits
   if ((double)nrows * (double)(ldx / 64) >= most || (double)N * (double)(ldw / 64) >= most) return OGL_EINVAL;
   if (M == 0 || N == 0) return OGL_OK;
