@@ -1009,9 +1009,8 @@ int gn_forward(const gn_args& A, const gn_plan& P, hipStream_t st) {
     if (P.even) GN_LAUNCH((k_gn_rows_fwd<T, V, NV, R, BLOCK, even>), grid);    \
     else GN_LAUNCH((k_gn_rows_fwd<T, V, NV, R, BLOCK, cut>), grid);            \
   } while (0)
-    if (P.block) {
-      if (P.nv == 1) GN_ROWS(1, 1, true);
-      else if (P.nv == 2) GN_ROWS(2, 1, true);
+    if (P.block) {                                                     // (more than 320 pieces: two a lane at least)
+      if (P.nv == 2) GN_ROWS(2, 1, true);
       else GN_ROWS(4, 1, true);
     } else {
       if (P.nv == 1 && P.r == 4) GN_ROWS(1, 4, false);
@@ -1060,10 +1059,10 @@ int gn_backward(const gn_args& A, const gn_plan& P, void* dw, void* db, hipStrea
     if (P.even) hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK, even>), grid, dim3(GN_THREADS), 0, st, A);      \
     else hipLaunchKernelGGL((k_gn_rows_bwd<T, V, NV, R, BLOCK, cut>), grid, dim3(GN_THREADS), 0, st, A);              \
   } while (0)
-    if (P.block) {
-      if (P.nv == 1) GN_ROWS(1, 1, true);
-      else if (P.nv == 2) GN_ROWS(2, 1, true);
-      else GN_ROWS(4, 1, true);
+    if (P.block) {                                                     // (more than 320 pieces, in 16-bit types 192)
+      if (P.nv == 2) GN_ROWS(2, 1, true);
+      else if (P.nv > 2) GN_ROWS(4, 1, true);
+      else if constexpr (V == 8) GN_ROWS(1, 1, true);
     } else {
       if (P.nv == 1 && P.r > 1) GN_ROWS(1, 2, false);
       else if (P.nv == 1) GN_ROWS(1, 1, false);
