@@ -73,3 +73,17 @@ def test_more_samples_than_blocks(ops, shape, G, dtype):
     check(ops, shape, G, dtype, act="silu", seed=shape[0])
     if dtype != torch.float32:
         check_sums(ops, shape, G, dtype, "silu", shape[0])
+
+
+# The other forms, once each: whole and cut pieces, 1 - 5 pieces a lane, the block as the team, few and many positions.
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape,G", [((70, 64), 2), ((9, 1024), 1), ((9, 1021), 1), ((9, 1200), 1), ((9, 1203), 1), ((9, 1600), 1), ((9, 1701), 1), ((9, 3200), 1),
+                                     ((9, 3203), 1), ((9, 4800), 1), ((9, 4803), 1), ((23303, 600), 30), ((65537, 256), 32), ((32771, 523), 1), ((32771, 528), 1),
+                                     ((2, 100, 75), 3), ((1, 3000, 75), 3), ((1500, 3, 27), 3)])
+def test_16_bit_forms(ops, dtype, shape, G):
+    check(ops, shape, G, dtype, act="silu", seed=sum(shape))
+
+
+@pytest.mark.parametrize("C", [1400, 1401, 4000, 4003])
+def test_float32_rows_of_a_block(ops, C):
+    check(ops, (9, C), 1, act="silu", seed=C)

@@ -1,16 +1,10 @@
-"""The int8 product's forms (few rows; tiles of 64, 128 and 256): the same arithmetic behind the exact sum in each."""
+"""The int8 product's forms (few rows; tiles of 64, 128 and 256): the same arithmetic behind the exact sum in each.  And the writes' forms."""
 import pytest
 import torch
 
+from test_gpu_int8 import check_cache, ops, oracle_rows  # noqa: F401
+
 pytestmark = pytest.mark.gpu
-
-
-@pytest.fixture(scope="module")
-def ops():
-    import ogl_amd  # noqa: F401
-    from ogl_amd import ops as _ops
-    assert torch.cuda.is_available(), "GPU tests need a GPU"
-    return _ops
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
@@ -33,3 +27,14 @@ def test_product_and_bias_are_rounded_once(ops, dtype, M, N, K):
     want = (p + bias.double()).float()
     assert float((want != 0).float().mean()) > 0.9
     assert torch.equal(ops.linear_int8(x, w, bias.contiguous(), dtype=dtype), want.to(dtype).expand(M, N))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_rows_of_every_number_of_pieces(ops, dtype, fmt):
+    """Rows of up to 10 pieces of 16 bytes a lane (5 in 16-bit types) and of a block, codes and scales equal to the definition's in 64 bits (quotients that
+    go through float32 on their way are not: 84.0000024 would become 84, the middle between two codes)."""
+    gen = torch.Generator().manual_seed(7)
+    for width in (1, 3, 7, 8, 15, 20, 33, 40, 48, 63, 65, 100, 130, 160, 250, 320, 602, 1000, 2000, 5121, 9000):
+        x = (torch.randn(5, width, generator=gen) * 3).to(dtype)
+        check_cache(ops.quantize_rows(x.cuda(), fmt=fmt), *oracle_rows(x, fmt, None))
