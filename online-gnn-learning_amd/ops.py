@@ -3599,6 +3599,8 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None)
     """``act(group_norm(x) * weight + bias)``, channels LAST: ``x`` [B, *spatial, C] in float32 / bfloat16 / float16, statistics over the positions of
     a sample and the C / num_groups channels of a group (a matrix [n, C]: over the channels of its row).  ``weight`` / ``bias`` [C] of the type of x
     or float32; ``activation`` None, 'relu', 'silu' or 'gelu' (x Phi(x)).  Statistics and sums are float32, each result is rounded once.
+    'silu' comes from the machine's exponential and reciprocal, (1.25 |z| + 4) 2^-24 of the value off at most (|z| <= 80); 'gelu' from a polynomial that is off by up to
+    3.2e-7 |z| (slope 4e-7): as near as float32 has it around zero and above, 5e-4 of the value at z = -4, 4e-3 at -6.
     Differentiable (once, in reverse mode) w.r.t. x, weight and bias; results do not depend on the run (no atomics)."""
     what = "group_norm"
     if x.dim() < 2:
