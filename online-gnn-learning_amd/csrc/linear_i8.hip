@@ -77,9 +77,10 @@ __device__ __forceinline__ void i8_out(const i8_args& A, int64_t m, int n, v4i32
 }
 
 // ---- few rows: every wave of a block takes a slice of K for the block's 16 output columns, straight from memory to the matrix unit ----------------
-// 16 weight rows x K a block, so N / 16 blocks; the weight is read once per MT * 16 rows of x and bounds the time: 16 x 12288, K = 4096 takes 14.5 us,
-// 3.5 TB/s of a weight that no cache holds (two steps a lane side by side, eight of them in flight, 4 or 16 waves and loads past the caches: the same
-// or slower).
+// 16 weight rows x K a block, so N / 16 blocks; the weight is read once per MT * 16 rows of x.  16 x 12288, K = 4096 takes 14.5 us, 3.5 TB/s of a weight
+// that no cache holds.  A step of a wave is its loads (the weight's and those of x), a wait for them and MT products: the loop is not unrolled, and the
+// waves of a CU have eight steps a block in flight between them.  Two steps at a time, 4 or 16 waves a block and loads past the caches took the same or
+// longer; more steps of a wave in flight have not been tried.
 template <typename T, int MT>
 __global__ void __launch_bounds__(512) k_i8_few(i8_args A) {
   constexpr int WAVES = 8;
@@ -98,7 +99,6 @@ __global__ void __launch_bounds__(512) k_i8_few(i8_args A) {
   v4i32 acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = v4i32{0, 0, 0, 0};
-#pragma unroll 4
   for (int k = wave; k < A.K64; k += WAVES) {
     const v4i32 a = *(const v4i32*)(wp + (int64_t)k * 64);
 #pragma unroll
