@@ -1,8 +1,9 @@
 #!/bin/bash
 # profiles/row_operators_kernel_stats.txt: kernel times of the row operators at the sizes of perf/operators.py, counters of those that take longest
-# (one run each: a run holds few counters), and the card's rates.  From the repository's root, with a GPU; the result is on stdout.
+# (one run each: a run holds few counters), and the card's rates.  From the repository's root, with a GPU: tools/collect_row_operators.sh FOLDER, which
+# takes the runs' raw output; the result is on stdout.
 set -e
-O=${1:-gpurun_out/row_operators}
+O=${1:?a folder for the runs}
 mkdir -p $O
 export TMPDIR=/tmp
 run() {   # case, kind, profiler's arguments (the profiler may end with 139 when all is done and written: the calls' last line counts then)
