@@ -18,7 +18,9 @@ LIB = os.path.join(HERE, "libogl_hip.so")
 OBJ_DIR = os.path.join(HERE, "build")
 # no packed fp32 instructions (v_pk_add / mul / fma_f32, which -O3 forms from ordinary float code): some of their forms have given wrong
 # results now and then on this part.  The scalar ones round the same.  (The host pass warns that it does not know the feature.)
-FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+# A loop request that the compiler cannot follow (an unroll that does not happen) is an error: the kernels' comments describe the loops as written.
+FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+         "-Werror=pass-failed"]
 
 
 def sources():
